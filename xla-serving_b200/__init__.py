@@ -9,6 +9,8 @@ fails if the CUDA library is missing.
 
 from . import _capi
 from . import dlrm
+from . import mx
+from . import experts
 from . import ops
 from . import sharding
 from ._capi import XseError

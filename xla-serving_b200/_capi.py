@@ -300,6 +300,60 @@ SIGNATURES.update({
 })
 
 
+# Microscaled 4-bit layers (include/xse_mx.h).
+class MxMatrixStruct(ctypes.Structure):
+  """xse_mx_matrix (include/xse_mx.h)."""
+  _fields_ = [
+      ("codes", ctypes.c_void_p),
+      ("scales", ctypes.c_void_p),
+      ("rows", ctypes.c_int64),
+      ("cols", ctypes.c_int32),
+      ("groups", ctypes.c_int32),
+  ]
+
+
+_MXP = ctypes.POINTER(MxMatrixStruct)
+SIGNATURES.update({
+    "xse_mxfp4_codes_bytes": (_I64, [_I64, _I32, _I32]),
+    "xse_mxfp4_scales_bytes": (_I64, [_I64, _I32, _I32]),
+    "xse_mxfp4_quantize": (_I, [_P, _I32, _I64, _I64, _I64, _MXP, _P]),
+    "xse_mxfp4_dequantize": (_I, [_MXP, _P, _I32, _I64, _I64, _P]),
+    "xse_linear_forward_mxfp4_q": (_I, [_MXP, _MXP, _P, _I32, _P, _I32, _I64,
+                                        _P]),
+    "xse_linear_mxfp4_workspace": (_I64, [_I64, _I32]),
+    "xse_linear_forward_mxfp4": (_I, [_P, _I32, _I64, _I64, _MXP, _P, _I32, _P,
+                                      _I32, _I64, _P, _I64, _P]),
+    "xse_mxfp4_check": (_I, [_P]),
+})
+
+
+# Expert sort, row movers and layers (include/xse_experts.h).
+class ExpertPlanStruct(ctypes.Structure):
+  """xse_expert_plan (include/xse_experts.h)."""
+  _fields_ = [
+      ("offsets", ctypes.c_void_p),
+      ("order", ctypes.c_void_p),
+      ("slots", ctypes.c_void_p),
+      ("tokens", ctypes.c_int64),
+      ("topk", ctypes.c_int32),
+      ("num_experts", ctypes.c_int32),
+  ]
+
+
+_PLANP = ctypes.POINTER(ExpertPlanStruct)
+SIGNATURES.update({
+    "xse_expert_sort": (_I, [_P, _I32, _PLANP, _P]),
+    "xse_expert_gather": (_I, [_P, _I32, _I32, _I64, _PLANP, _P, _I64, _P]),
+    "xse_expert_combine": (_I, [_P, _I32, _I32, _I64, _PLANP, _P, _P, _I64,
+                                _P]),
+    "xse_expert_combine_backward": (_I, [_P, _P, _I32, _I32, _I64, _I64,
+                                         _PLANP, _P, _P, _I64, _P, _P]),
+    "xse_expert_linear_workspace": (_I64, [_I64, _I32, _I32]),
+    "xse_expert_linear_mxfp4": (_I, [_P, _I32, _I64, _I32, _PLANP, _MXP, _P,
+                                     _I32, _P, _I32, _I64, _P, _I64, _P]),
+})
+
+
 def _load():
   if not os.path.exists(LIB_PATH):
     raise ImportError(

@@ -1,0 +1,959 @@
+// Products of microscaled 4-bit matrices (include/xse_mx.h,
+// include/xse_experts.h) on the fifth-generation tensor cores.
+//
+//   y[r][f] = act(sum_k x[r][k] w[f][k] + bias[f])
+//
+// with x and w as E2M1 codes and one power-of-two scale per 32 elements of k.
+// tcgen05.mma kind::mxf4 multiplies the codes, applies both scales of each
+// block of 32 and accumulates in fp32 in tensor memory.
+//
+// Roles. The weights are the MMA's A operand (128 features, the lanes of the
+// accumulator) and the rows its B operand (kN rows, the accumulator's columns)
+// for every size: a handful of rows then wastes no tensor-core rows, and the
+// epilogue's warps hold 32 neighbouring features of a row, so that y is
+// written in whole sectors without a transposition.
+//
+// One block per SM runs over its tiles: warp 0 copies stages of 256 elements
+// of k with TMA (codes, 128-byte swizzled; scales, 512-byte tiles as they lie
+// in memory), warp 1 moves the scales to tensor memory and issues the MMAs,
+// warps 2 to 5 write the previous tile's results from the second accumulator.
+//
+// Few tiles: a cluster of `split` blocks shares a tile, each taking a part of
+// k; the parts are added in block order over distributed shared memory.
+//
+// Every wait is bounded. One that runs out sets a flag that the other roles
+// see and g_wait_failed, which xse_mxfp4_check reports.
+
+#include <cuda.h>
+
+#include <cstring>
+#include <mutex>
+
+#include "../../include/xse_dlrm.h"
+#include "xse_mx_internal.h"
+
+namespace xse {
+namespace {
+
+constexpr int kM = 128;            // features of a tile
+constexpr int kStageK = 256;       // elements of k per stage (128 bytes)
+constexpr int kThreads = 192;
+constexpr int kEpilogueWarps = 4;
+constexpr int kABytes = kM * kStageK / 2;
+constexpr int kScaleBytes = 2 * kMxTileBytes;  // a tile row's, per stage
+constexpr long long kWaitCycles = 4000000000ll;  // about two seconds
+
+__device__ int g_wait_failed;
+
+template <int kN>
+struct Config {
+  static constexpr int kBBytes = kN * kStageK / 2;
+  static constexpr int kBTiles = kN <= 128 ? 1 : 2;  // scale tiles of b
+  static constexpr int kStageBytes =
+      kABytes + kBBytes + kScaleBytes * (1 + kBTiles);
+  static constexpr int kMost = (204 * 1024) / kStageBytes;
+  static constexpr int kStages = kMost > 10 ? 10 : kMost;
+  // Tensor memory columns: accumulators, then each stage's scales.
+  static constexpr int kAccColumns = kN < 32 ? 32 : kN;
+  static constexpr int kAccs = kN <= 192 ? 2 : 1;
+  static constexpr int kScaleColumns = 8 * (1 + kBTiles);
+  static_assert(kAccs * kAccColumns + kStages * kScaleColumns <= 512,
+                "tensor memory");
+};
+
+struct GemmParams {
+  CUtensorMap a;  // weights [groups][out][row bytes]
+  CUtensorMap b;  // rows [rows][row bytes]
+  const uint8_t* a_scales;
+  const uint8_t* b_scales;
+  const float* bias;
+  void* y;
+  const int32_t* offsets;  // expert rows, or NULL for one group of all rows
+  int64_t y_stride;
+  int64_t rows;            // of b (and y)
+  int64_t b_tiles;         // scale tiles of b, of kN rows or more
+  int32_t groups;
+  int32_t out;
+  int32_t k;
+  int32_t k_tiles;
+  int32_t k_stages;
+  int32_t m_tiles;
+  int32_t activation;
+  int32_t y_bf16;
+  int32_t split;           // blocks of a cluster that share a tile's k
+};
+
+// ---------------------------------------------------------------- PTX forms
+
+__device__ __forceinline__ uint32_t SharedAddress(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+__device__ __forceinline__ void BarrierInit(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)
+               : "memory");
+}
+
+__device__ __forceinline__ void BarrierExpect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                   bar), "r"(bytes)
+               : "memory");
+}
+
+__device__ __forceinline__ void BarrierArrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ bool BarrierTry(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+// False when the wait ran out, here or (as `failed` tells) in another role.
+__device__ __forceinline__ bool BarrierWait(uint32_t bar, uint32_t parity,
+                                            volatile int* failed) {
+  if (BarrierTry(bar, parity)) return true;
+  const long long begin = clock64();
+  while (!BarrierTry(bar, parity)) {
+    if (*failed) return false;
+    if (clock64() - begin > kWaitCycles) {
+      *failed = 1;
+      g_wait_failed = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void TmaLoad3(uint32_t dst, const CUtensorMap* map,
+                                         int x, int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::"
+      "complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void TmaLoad2(uint32_t dst, const CUtensorMap* map,
+                                         int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::"
+      "complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void BulkLoad(uint32_t dst, const void* src,
+                                         uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes "
+      "[%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+__device__ __forceinline__ void FenceAfterSync() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void FenceBeforeSync() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+
+// Arrives at `bar` once the MMAs and copies issued so far are done.
+__device__ __forceinline__ void Commit(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 "
+      "[%0];" ::"r"(bar)
+      : "memory");
+}
+
+// 512 bytes of scales (32 rows of 16 bytes, in shared memory as 8-row groups
+// of 128 bytes) to four columns, repeated for each warp's lanes.
+__device__ __forceinline__ void CopyScales(uint32_t column, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(column),
+               "l"(desc)
+               : "memory");
+}
+
+__device__ __forceinline__ void Mma(uint32_t acc, uint64_t a, uint64_t b,
+                                    uint32_t idesc, uint32_t a_scales,
+                                    uint32_t b_scales, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X "
+      "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales),
+      "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+template <int kColumns>
+__device__ __forceinline__ void LoadColumns(uint32_t address,
+                                            float (&v)[kColumns]) {
+  static_assert(kColumns == 16, "one instruction");
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, "
+      "%8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+        "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(address)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ void ClusterSync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ float LoadPeer(uint32_t address, int rank) {
+  uint32_t remote;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(remote)
+               : "r"(address), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote)
+               : "memory");
+  return v;
+}
+
+// Shared memory descriptors (addresses and strides in 16-byte units, version
+// 1): K-major rows of 128 bytes with the 128-byte swizzle, 1024 bytes between
+// groups of 8 rows; and unswizzled 8 x 16-byte groups, 128 bytes apart.
+__device__ __forceinline__ uint64_t SwizzledDesc(uint32_t address) {
+  return static_cast<uint64_t>((address >> 4) & 0x3fff) | (1ull << 16) |
+         (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ uint64_t ScaleDesc(uint32_t address) {
+  return static_cast<uint64_t>((address >> 4) & 0x3fff) | (1ull << 16) |
+         (8ull << 32) | (1ull << 46);
+}
+
+// Instruction descriptor of kind::mxf4: E2M1 x E2M1, E8M0 scales, K-major
+// operands, dense; `half` selects the scale bytes 0-1 or 2-3 of a column.
+template <int kN>
+__device__ __forceinline__ uint32_t InstructionDesc(uint32_t half) {
+  const uint32_t id = half * 2;
+  return (id << 4) | (1u << 7) | (1u << 10) |
+         (static_cast<uint32_t>(kN / 8) << 17) | (1u << 23) |
+         (static_cast<uint32_t>(kM / 16) << 24) | (id << 29);
+}
+
+// -------------------------------------------------------------------- tiles
+
+struct Tile {
+  int group;       // weights' group
+  int64_t row;     // first row of b and y
+  int rows;        // of the tile that exist
+  int m;           // feature tile
+  int64_t b_tile;  // first scale tile of b
+};
+
+// Groups' first row tiles (a running count) and rows in shared memory.
+template <int kN>
+__device__ __forceinline__ Tile TileOf(const GemmParams& p, int64_t item,
+                                       const int* tile_begin,
+                                       const int* row_begin) {
+  using C = Config<kN>;
+  Tile t;
+  const int64_t n = item / p.m_tiles;
+  t.m = static_cast<int>(item - n * p.m_tiles);
+  t.group = 0;
+  int64_t at = n;
+  int64_t first = 0, count = p.rows;
+  if (p.offsets != nullptr) {
+    int low = 0, high = p.groups - 1;  // the last group that begins by n
+    while (low < high) {
+      const int mid = (low + high + 1) / 2;
+      if (tile_begin[mid] <= n) {
+        low = mid;
+      } else {
+        high = mid - 1;
+      }
+    }
+    t.group = low;
+    at = n - tile_begin[low];
+    first = row_begin[low];
+    count = row_begin[low + 1] - first;
+  }
+  t.row = first + at * kN;
+  const int64_t left = count - at * kN;
+  t.rows = static_cast<int>(left < kN ? left : kN);
+  t.b_tile = first / kN + t.group + at * C::kBTiles;
+  return t;
+}
+
+__device__ __forceinline__ float Activate(float v, int activation) {
+  if (activation == XSE_ACT_RELU) return v < 0.0f ? 0.0f : v;  // keeps NaN
+  if (activation == XSE_ACT_SIGMOID) return 1.0f / (1.0f + expf(-v));
+  return v;
+}
+
+__device__ __forceinline__ void StoreY(const GemmParams& p, int64_t row,
+                                       int feature, float v) {
+  if (p.y_bf16) {
+    static_cast<__nv_bfloat16*>(p.y)[row * p.y_stride + feature] =
+        __float2bfloat16_rn(v);
+  } else {
+    static_cast<float*>(p.y)[row * p.y_stride + feature] = v;
+  }
+}
+
+template <int kN>
+__global__ void __launch_bounds__(kThreads, 1)
+    MxGemmKernel(const __grid_constant__ GemmParams p) {
+  using C = Config<kN>;
+  extern __shared__ uint8_t raw[];
+  __shared__ alignas(8) uint64_t full_bar[C::kStages];
+  __shared__ alignas(8) uint64_t empty_bar[C::kStages];
+  __shared__ alignas(8) uint64_t acc_full_bar[2];
+  __shared__ alignas(8) uint64_t acc_empty_bar[2];
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int failed;
+  __shared__ int scan_carry;  // row tiles of all groups
+
+  uint8_t* stages = raw + (1024 - (SharedAddress(raw) & 1023)) % 1024;
+  int* tile_begin =
+      reinterpret_cast<int*>(stages + C::kStages * C::kStageBytes);
+  int* row_begin = tile_begin + (p.groups + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int rank = static_cast<int>(blockIdx.x) % p.split;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      BarrierInit(SharedAddress(full_bar + i), 1);
+      BarrierInit(SharedAddress(empty_bar + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      BarrierInit(SharedAddress(acc_full_bar + i), 1);
+      BarrierInit(SharedAddress(acc_empty_bar + i), kEpilogueWarps);
+    }
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile(
+        "tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;"
+        ::"r"(SharedAddress(&tmem_base))
+        : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;"
+                 ::: "memory");
+  }
+  if (p.offsets != nullptr && warp == 2) {
+    // The plan's offsets, held to [0, rows], and a scan of the row tiles.
+    int carry = 0;
+    for (int base = 0; base <= p.groups; base += 32) {
+      const int i = base + lane;
+      const int rows = static_cast<int>(p.rows);
+      int begin = 0, end = 0;
+      if (i <= p.groups) {
+        begin = min(max(__ldg(p.offsets + i), 0), rows);
+        row_begin[i] = begin;
+      }
+      if (i < p.groups) end = min(max(__ldg(p.offsets + i + 1), 0), rows);
+      int tiles = end > begin && i < p.groups ? (end - begin + kN - 1) / kN : 0;
+      int scan = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += up;
+      }
+      if (i <= p.groups) tile_begin[i] = carry + scan - tiles;
+      carry += __shfl_sync(0xffffffffu, scan, 31);
+    }
+    if (lane == 0) scan_carry = carry;
+  }
+  FenceBeforeSync();
+  __syncthreads();
+  FenceAfterSync();
+  const uint32_t tmem = tmem_base;
+  const int64_t row_tiles =
+      p.offsets != nullptr ? scan_carry : (p.rows + kN - 1) / kN;
+  const int64_t items = row_tiles * p.m_tiles;
+  const int64_t first_item = blockIdx.x / p.split;
+  const int64_t item_step = gridDim.x / p.split;
+  // This block's part of k, in stages.
+  const int k_begin = static_cast<int>(
+      static_cast<int64_t>(p.k_stages) * rank / p.split);
+  const int k_end = static_cast<int>(
+      static_cast<int64_t>(p.k_stages) * (rank + 1) / p.split);
+  const uint32_t stage_base = SharedAddress(stages);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int64_t issued = 0;
+      for (int64_t item = first_item; ok && item < items; item += item_step) {
+        const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+        const uint8_t* a_scales =
+            p.a_scales + (static_cast<int64_t>(t.group) * p.m_tiles + t.m) *
+                             p.k_tiles * kMxTileBytes;
+        const uint8_t* b_scales =
+            p.b_scales + t.b_tile * p.k_tiles * kMxTileBytes;
+        const bool b_first = t.b_tile < p.b_tiles;
+        const bool b_second = C::kBTiles == 2 && t.b_tile + 1 < p.b_tiles;
+        for (int s = k_begin; s < k_end; ++s) {
+          const uint32_t bar = SharedAddress(full_bar + stage);
+          ok = BarrierWait(SharedAddress(empty_bar + stage), phase ^ 1,
+                           &failed);
+          if (!ok) break;
+          const uint32_t at = stage_base + stage * C::kStageBytes;
+          const uint32_t scales = at + kABytes + C::kBBytes;
+          const uint32_t bytes =
+              2 * s + 1 < p.k_tiles ? kScaleBytes : kMxTileBytes;
+          BarrierExpect(bar, kABytes + C::kBBytes +
+                                 bytes * (1 + b_first + b_second));
+          TmaLoad3(at, &p.a, s * (kStageK / 2), t.m * kM, t.group, bar);
+          TmaLoad2(at + kABytes, &p.b, s * (kStageK / 2),
+                   static_cast<int>(t.row), bar);
+          const int64_t k_at = static_cast<int64_t>(2 * s) * kMxTileBytes;
+          BulkLoad(scales, a_scales + k_at, bytes, bar);
+          if (b_first) {
+            BulkLoad(scales + kScaleBytes, b_scales + k_at, bytes, bar);
+          }
+          if (b_second) {
+            BulkLoad(scales + 2 * kScaleBytes,
+                     b_scales + p.k_tiles * kMxTileBytes + k_at, bytes, bar);
+          }
+          ++issued;
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // After a failure the copies in flight still have to land.
+      if (!ok) {
+        volatile int ignored = 0;
+        const int in_flight =
+            static_cast<int>(issued < C::kStages ? issued : C::kStages);
+        for (int i = 0; i < in_flight; ++i) {
+          if (--stage < 0) {
+            stage = C::kStages - 1;
+            phase ^= 1;
+          }
+          BarrierWait(SharedAddress(full_bar + stage), phase, &ignored);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int64_t item = first_item; ok && item < items; item += item_step) {
+        const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+        ok = BarrierWait(SharedAddress(acc_empty_bar + acc), acc_phase ^ 1,
+                         &failed);
+        if (!ok) break;
+        FenceAfterSync();
+        const uint32_t d = tmem + acc * C::kAccColumns;
+        for (int s = k_begin; s < k_end; ++s) {
+          ok = BarrierWait(SharedAddress(full_bar + stage), phase, &failed);
+          if (!ok) break;
+          FenceAfterSync();
+          const uint32_t at = stage_base + stage * C::kStageBytes;
+          const uint32_t scales = at + kABytes + C::kBBytes;
+          // The stage's own columns: they are free once its last MMAs are
+          // done, which the stage's empty barrier has shown.
+          const uint32_t a_col =
+              tmem + C::kAccs * C::kAccColumns + stage * C::kScaleColumns;
+          const uint32_t b_col = a_col + 8;
+          const int left = p.k - s * kStageK;
+          const int steps = left >= kStageK ? 4 : (left + 63) / 64;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h * 2 >= steps) break;
+            CopyScales(a_col + h * 4, ScaleDesc(scales + h * kMxTileBytes));
+#pragma unroll
+            for (int q = 0; q < C::kBTiles; ++q) {
+              CopyScales(b_col + (h * C::kBTiles + q) * 4,
+                         ScaleDesc(scales + (1 + q) * kScaleBytes +
+                                   h * kMxTileBytes));
+            }
+          }
+          for (int j = 0; j < steps; ++j) {
+            Mma(d, SwizzledDesc(at + j * 32),
+                SwizzledDesc(at + kABytes + j * 32),
+                InstructionDesc<kN>(j & 1), a_col + (j >> 1) * 4,
+                b_col + (j >> 1) * 4 * C::kBTiles,
+                s > k_begin || j > 0);
+          }
+          Commit(SharedAddress(empty_bar + stage));
+          if (++stage == C::kStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        Commit(SharedAddress(acc_full_bar + acc));
+        if (++acc == C::kAccs) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+    }
+  } else {
+    // Tensor memory lanes [32 q, 32 q + 32) belong to warps with warp % 4 = q.
+    const int quarter = warp & 3;
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int64_t item = first_item; item < items; item += item_step) {
+      const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+      const bool ok = BarrierWait(SharedAddress(acc_full_bar + acc), acc_phase,
+                                  &failed);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      FenceAfterSync();
+      const int feature = t.m * kM + quarter * 32 + lane;
+      const bool mine = feature < p.out;
+      const uint32_t d = tmem + acc * C::kAccColumns +
+                         (static_cast<uint32_t>(quarter * 32) << 16);
+      const float bias =
+          p.bias != nullptr && mine
+              ? __ldg(p.bias + static_cast<int64_t>(t.group) * p.out + feature)
+              : 0.0f;
+      if (p.split == 1) {
+        for (int c = 0; c < kN && c < t.rows; c += 16) {
+          float v[16];
+          LoadColumns<16>(d + c, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (mine && c + i < t.rows) {
+              StoreY(p, t.row + c + i, feature,
+                     Activate(v[i] + bias, p.activation));
+            }
+          }
+        }
+      } else {
+        // This block's part, [column][feature], over the stages (all read).
+        float* part = reinterpret_cast<float*>(stages);
+        for (int c = 0; c < kN && c < t.rows; c += 16) {
+          float v[16];
+          LoadColumns<16>(d + c, v);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            part[(c + i) * kM + quarter * 32 + lane] =
+                k_end > k_begin ? v[i] : 0.0f;
+          }
+        }
+      }
+      FenceBeforeSync();
+      __syncwarp();
+      if (lane == 0) BarrierArrive(SharedAddress(acc_empty_bar + acc));
+      if (++acc == C::kAccs) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    // Rows behind the last group's.
+    if (p.offsets != nullptr) {
+      const int64_t kept = row_begin[p.groups];
+      const int64_t total = (p.rows - kept) * p.out;
+      const int thread = threadIdx.x - 64;
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + thread;
+           i < total; i += static_cast<int64_t>(gridDim.x) * 128) {
+        const int64_t r = i / p.out;
+        StoreY(p, kept + r, static_cast<int>(i - r * p.out), 0.0f);
+      }
+    }
+  }
+  if (p.split > 1) {
+    // One tile per cluster; all its blocks come here, also without a tile.
+    __syncwarp();
+    ClusterSync();
+    if (warp >= 2 && first_item < items && !failed) {
+      const Tile t = TileOf<kN>(p, first_item, tile_begin, row_begin);
+      const int lane_feature = (warp & 3) * 32 + lane;
+      const int feature = t.m * kM + lane_feature;
+      const float bias =
+          p.bias != nullptr && feature < p.out
+              ? __ldg(p.bias + static_cast<int64_t>(t.group) * p.out + feature)
+              : 0.0f;
+      for (int c = rank; c < t.rows; c += p.split) {
+        const uint32_t at = stage_base + (c * kM + lane_feature) * 4;
+        float sum = 0.0f;
+        for (int b = 0; b < p.split; ++b) sum += LoadPeer(at, b);
+        if (feature < p.out) {
+          StoreY(p, t.row + c, feature, Activate(sum + bias, p.activation));
+        }
+      }
+    }
+    __syncwarp();
+    ClusterSync();
+  }
+  __syncwarp();
+  FenceBeforeSync();
+  __syncthreads();
+  if (warp == 1) {
+    FenceAfterSync();
+    asm volatile(
+        "tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem)
+        : "memory");
+  }
+}
+
+// ------------------------------------------------------------------- launch
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
+                                 void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+
+EncodeTiled GetEncodeTiled() {
+  static EncodeTiled fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000,
+                                         cudaEnableDefault,
+                                         &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      p = nullptr;
+    }
+    return reinterpret_cast<EncodeTiled>(p);
+  }();
+  return fn;
+}
+
+// [groups][rows][row bytes] of codes as boxes of 128 bytes x `box_rows`,
+// swizzled; parts of a box outside the matrix read as zero codes.
+int EncodeCodes(CUtensorMap* map, const void* codes, int64_t row_bytes,
+                int64_t rows, int64_t groups, int rank, int box_rows) {
+  EncodeTiled encode = GetEncodeTiled();
+  if (encode == nullptr) {
+    return FailWith(XSE_INTERNAL, "cuTensorMapEncodeTiled is not available");
+  }
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(row_bytes),
+                              static_cast<cuuint64_t>(rows),
+                              static_cast<cuuint64_t>(groups)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_bytes),
+                                 static_cast<cuuint64_t>(row_bytes * rows)};
+  const cuuint32_t box[3] = {kStageK / 2, static_cast<cuuint32_t>(box_rows),
+                             1};
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = encode(
+      map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(codes), dims,
+      strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return FailWith(XSE_INTERNAL, "tensor map of 4-bit codes: error %d",
+                    static_cast<int>(r));
+  }
+  return XSE_OK;
+}
+
+template <int kN>
+int LaunchGemm(GemmParams& p, int64_t codes_rows, const void* a_codes,
+               const void* b_codes, int64_t most_items, cudaStream_t s) {
+  using C = Config<kN>;
+  const int64_t row_bytes = MxRowBytes(p.k);
+  int rc = EncodeCodes(&p.a, a_codes, row_bytes, p.out, p.groups, 3, kM);
+  if (rc == XSE_OK) {
+    rc = EncodeCodes(&p.b, b_codes, row_bytes, codes_rows, 1, 2, kN);
+  }
+  if (rc != XSE_OK) return rc;
+  const size_t smem = 1024 + C::kStages * C::kStageBytes +
+                      (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
+  cudaError_t e = cudaFuncSetAttribute(
+      MxGemmKernel<kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      static_cast<int>(smem));
+  if (e == cudaSuccess) {
+    int64_t blocks = most_items * p.split;
+    if (p.split == 1 && blocks > kNumSms) blocks = kNumSms;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(blocks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(p.split);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, MxGemmKernel<kN>, p);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return FailWith(XSE_INTERNAL, "4-bit product launch: %s",
+                    cudaGetErrorString(e));
+  }
+  return XSE_OK;
+}
+
+// The product of rows in b (codes, scales) with w; plan NULL: one group.
+int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
+            int64_t b_tiles, const xse_mx_matrix& w, const float* bias,
+            int32_t activation, const xse_expert_plan* plan, void* y,
+            int32_t y_dtype, int64_t y_stride, cudaStream_t s) {
+  GemmParams p{};
+  p.a_scales = static_cast<const uint8_t*>(w.scales);
+  p.b_scales = static_cast<const uint8_t*>(b_scales);
+  p.bias = bias;
+  p.y = y;
+  p.offsets = plan != nullptr ? plan->offsets : nullptr;
+  p.y_stride = y_stride;
+  p.rows = rows;
+  p.b_tiles = b_tiles;
+  p.groups = plan != nullptr ? plan->num_experts : 1;
+  p.out = static_cast<int32_t>(w.rows);
+  p.k = w.cols;
+  p.k_tiles = static_cast<int32_t>(MxKTiles(w.cols));
+  p.k_stages = (w.cols + kStageK - 1) / kStageK;
+  p.m_tiles = static_cast<int32_t>(MxRowTiles(w.rows));
+  p.activation = activation;
+  p.y_bf16 = y_dtype == XSE_DT_BF16;
+  p.split = 1;
+  // Rows a group has on average decide the tile's rows.
+  const int n = MxTileRowsFor(rows, p.groups);
+  const int64_t row_tiles =
+      plan == nullptr ? (rows + n - 1) / n
+                      : rows / n + (p.groups < rows ? p.groups : rows);
+  const int64_t items = row_tiles * p.m_tiles;
+  // A tile's k is shared where whole tiles would leave SMs idle.
+  if (n <= 64) {
+    while (p.split < 8 && items * p.split * 2 <= kNumSms &&
+           p.split * 2 <= p.k_stages) {
+      p.split *= 2;
+    }
+  }
+  switch (n) {
+    case 16:
+      return LaunchGemm<16>(p, rows, w.codes, b_codes, items, s);
+    case 32:
+      return LaunchGemm<32>(p, rows, w.codes, b_codes, items, s);
+    case 64:
+      return LaunchGemm<64>(p, rows, w.codes, b_codes, items, s);
+    default:
+      return LaunchGemm<128>(p, rows, w.codes, b_codes, items, s);
+  }
+}
+
+int CheckLayer(const xse_mx_matrix* w, int32_t activation, int32_t y_dtype,
+               int64_t y_stride) {
+  if (int rc = CheckMxMatrix(w, "w"); rc != XSE_OK) return rc;
+  if (w->rows < 1) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit matrix w needs at least one output row.");
+  }
+  if (activation < XSE_ACT_NONE || activation > XSE_ACT_SIGMOID) {
+    return FailWith(XSE_INVALID_ARGUMENT, "Unknown activation: %d",
+                    activation);
+  }
+  if (y_dtype != XSE_DT_F32 && y_dtype != XSE_DT_BF16) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layers write float32 or bfloat16, got type %d",
+                    y_dtype);
+  }
+  if (y_stride < w->rows) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer needs an output row stride >= out.");
+  }
+  return XSE_OK;
+}
+
+int CheckRowsIn(const void* x, int32_t x_dtype, int64_t rows, int64_t x_stride,
+                int32_t in_dim, const void* workspace, int64_t have,
+                int64_t need) {
+  if (x_dtype != XSE_DT_F32 && x_dtype != XSE_DT_BF16) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layers read float32 or bfloat16, got type %d",
+                    x_dtype);
+  }
+  if (rows < 0 || rows > INT32_MAX || x_stride < in_dim) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer needs 0 <= rows < 2^31 and an input row "
+                    "stride >= in.");
+  }
+  if (rows > 0 && (x == nullptr || workspace == nullptr)) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer buffers must be non-null.");
+  }
+  if (rows > 0 && (have < need || !Aligned16(workspace))) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer needs a 16-byte aligned workspace of %lld "
+                    "bytes, got %lld.", static_cast<long long>(need),
+                    static_cast<long long>(have));
+  }
+  return XSE_OK;
+}
+
+}  // namespace
+}  // namespace xse
+
+extern "C" {
+
+int xse_linear_forward_mxfp4_q(const xse_mx_matrix* x, const xse_mx_matrix* w,
+                               const float* bias, int32_t activation, void* y,
+                               int32_t y_dtype, int64_t y_stride,
+                               void* stream) {
+  using namespace xse;
+  SetLastLaunchCount(0);
+  if (int rc = CheckLayer(w, activation, y_dtype, y_stride); rc != XSE_OK) {
+    return rc;
+  }
+  if (int rc = CheckMxMatrix(x, "x"); rc != XSE_OK) return rc;
+  if (x->groups != 1 || w->groups != 1 || x->cols != w->cols) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer needs x and w of one group and of equal "
+                    "columns, got %d and %d.", x->cols, w->cols);
+  }
+  if (x->rows == 0) return XSE_OK;
+  if (y == nullptr) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer buffers must be non-null.");
+  }
+  const int rc =
+      RunGemm(x->codes, x->scales, x->rows, MxRowTiles(x->rows), *w, bias,
+              activation, nullptr, y, y_dtype, y_stride,
+              static_cast<cudaStream_t>(stream));
+  if (rc == XSE_OK) SetLastLaunchCount(1);
+  return rc;
+}
+
+int64_t xse_linear_mxfp4_workspace(int64_t rows, int32_t in_dim) {
+  return xse_mxfp4_codes_bytes(rows, in_dim, 1) +
+         xse_mxfp4_scales_bytes(rows, in_dim, 1);
+}
+
+int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
+                             int64_t x_stride, const xse_mx_matrix* w,
+                             const float* bias, int32_t activation, void* y,
+                             int32_t y_dtype, int64_t y_stride,
+                             void* workspace, int64_t workspace_bytes,
+                             void* stream) {
+  using namespace xse;
+  SetLastLaunchCount(0);
+  if (int rc = CheckLayer(w, activation, y_dtype, y_stride); rc != XSE_OK) {
+    return rc;
+  }
+  if (w->groups != 1) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer needs w of one group, got %d.", w->groups);
+  }
+  if (int rc = CheckRowsIn(x, x_dtype, rows, x_stride, w->cols, workspace,
+                           workspace_bytes,
+                           xse_linear_mxfp4_workspace(rows, w->cols));
+      rc != XSE_OK) {
+    return rc;
+  }
+  if (rows == 0) return XSE_OK;
+  if (y == nullptr) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer buffers must be non-null.");
+  }
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + xse_mxfp4_codes_bytes(rows, w->cols, 1);
+  int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, nullptr, false,
+                        codes, scales, s);
+  if (rc == XSE_OK) {
+    rc = RunGemm(codes, scales, rows, MxRowTiles(rows), *w, bias, activation,
+                 nullptr, y, y_dtype, y_stride, s);
+  }
+  if (rc == XSE_OK) SetLastLaunchCount(2);
+  return rc;
+}
+
+int64_t xse_expert_linear_workspace(int64_t pairs, int32_t num_experts,
+                                    int32_t in_dim) {
+  if (pairs < 0 || pairs > INT32_MAX || num_experts < 1 ||
+      num_experts > XSE_MAX_EXPERTS || in_dim < 1) {
+    return 0;
+  }
+  const int n = xse::MxTileRowsFor(pairs, num_experts);
+  return pairs * xse::MxRowBytes(in_dim) +
+         xse::ExpertScaleTiles(pairs, num_experts, n) *
+             xse::MxKTiles(in_dim) * xse::kMxTileBytes;
+}
+
+int xse_expert_linear_mxfp4(const void* x, int32_t x_dtype, int64_t x_stride,
+                            int32_t sorted, const xse_expert_plan* plan,
+                            const xse_mx_matrix* w, const float* bias,
+                            int32_t activation, void* y, int32_t y_dtype,
+                            int64_t y_stride, void* workspace,
+                            int64_t workspace_bytes, void* stream) {
+  using namespace xse;
+  SetLastLaunchCount(0);
+  if (int rc = CheckExpertPlan(plan); rc != XSE_OK) return rc;
+  if (int rc = CheckLayer(w, activation, y_dtype, y_stride); rc != XSE_OK) {
+    return rc;
+  }
+  if (w->groups != plan->num_experts) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "Expert layer needs one group of w per expert: %d groups, "
+                    "%d experts.", w->groups, plan->num_experts);
+  }
+  const int64_t pairs = plan->tokens * plan->topk;
+  const int64_t rows = sorted ? pairs : plan->tokens;
+  if (int rc = CheckRowsIn(x, x_dtype, rows, x_stride, w->cols, workspace,
+                           workspace_bytes,
+                           xse_expert_linear_workspace(
+                               pairs, plan->num_experts, w->cols));
+      rc != XSE_OK) {
+    return rc;
+  }
+  if (pairs == 0) return XSE_OK;
+  if (y == nullptr) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "4-bit layer buffers must be non-null.");
+  }
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  uint8_t* codes = static_cast<uint8_t*>(workspace);
+  uint8_t* scales = codes + pairs * MxRowBytes(w->cols);
+  int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, plan, sorted != 0,
+                        codes, scales, s);
+  if (rc == XSE_OK) {
+    rc = RunGemm(codes, scales, pairs,
+                 ExpertScaleTiles(pairs, plan->num_experts,
+                                  MxTileRowsFor(pairs, plan->num_experts)),
+                 *w, bias, activation, plan, y, y_dtype, y_stride, s);
+  }
+  if (rc == XSE_OK) SetLastLaunchCount(2);
+  return rc;
+}
+
+int xse_mxfp4_check(void* stream) {
+  using namespace xse;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int failed = 0;
+  cudaError_t e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) {
+    e = cudaMemcpyFromSymbol(&failed, g_wait_failed, sizeof(failed));
+  }
+  if (e == cudaSuccess && failed != 0) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_wait_failed, &zero, sizeof(zero));
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return FailWith(XSE_INTERNAL, "4-bit product check: %s",
+                    cudaGetErrorString(e));
+  }
+  if (failed != 0) {
+    return FailWith(XSE_DEADLINE_EXCEEDED,
+                    "A wait in a 4-bit product's kernel ran out.");
+  }
+  return XSE_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,147 @@
+// Shared by the 4-bit and expert kernels: argument checks, the microscaled
+// layout (include/xse_mx.h) and its device-side conversions.
+#ifndef XSE_MX_INTERNAL_H_
+#define XSE_MX_INTERNAL_H_
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/xse_emb.h"
+#include "../../include/xse_experts.h"
+#include "../../include/xse_mx.h"
+#include "xse_internal.h"
+
+namespace xse {
+
+constexpr int kMxBlock = 32;       // elements per scale
+constexpr int kMxTileRows = 128;   // rows of a scale tile
+constexpr int kMxTileBytes = 512;  // 128 rows x 4 blocks
+constexpr int kNumSms = 148;
+
+// Sets the error text (printf style) and returns `code`.
+int FailWith(int code, const char* fmt, ...)
+    __attribute__((format(printf, 2, 3)));
+// XSE_OK, or XSE_INTERNAL with the pending launch error of `what`.
+int LaunchStatus(const char* what);
+
+inline int64_t MxRowBytes(int64_t cols) { return (cols + 31) / 32 * 16; }
+inline int64_t MxKTiles(int64_t cols) { return (cols + 127) / 128; }
+inline int64_t MxRowTiles(int64_t rows) { return (rows + 127) / 128; }
+
+inline bool Aligned16(const void* p) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+
+// XSE_OK for a usable matrix of `what`; buffers are checked unless empty.
+int CheckMxMatrix(const xse_mx_matrix* q, const char* what);
+// XSE_OK for a usable plan (arrays non-null where they have entries).
+int CheckExpertPlan(const xse_expert_plan* plan);
+
+// Rows of a product's tile for groups of rows / groups rows on average. The
+// scales of an expert product's rows are laid out in 512-byte tiles of that
+// many rows each, so that every tile's scales begin a column of tensor memory.
+inline int MxTileRowsFor(int64_t rows, int32_t groups) {
+  const int64_t mean = (rows + groups - 1) / groups;
+  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+}
+
+// Scale tiles of n rows that hold every expert's rows on tile boundaries:
+// expert e's rows start at tile offsets[e] / n + e. With c rows it ends by
+// tile offsets[e] / n + e + ceil(c / n) <= (offsets[e] + c) / n + e + 1, the
+// next one's start, so no scan of the counts is needed.
+inline int64_t ExpertScaleTiles(int64_t pairs, int32_t num_experts, int n) {
+  return pairs / n + num_experts;
+}
+
+// Quantises the rows of x for a product: plan NULL as xse_mxfp4_quantize of
+// one contiguous-row group; else to the sorted rows' places (codes by sorted
+// row, scales as ExpertScaleTiles says), from token rows or sorted ones.
+int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
+                 int64_t row_stride, const xse_expert_plan* plan, bool sorted,
+                 void* codes, void* scales, cudaStream_t stream);
+
+#ifdef __CUDACC__
+
+// The E8M0 byte of a block whose largest magnitude has these bits.
+__device__ __forceinline__ uint32_t MxScaleByte(uint32_t amax_bits) {
+  const uint32_t e = amax_bits >> 23;
+  if (e == 255u) return 255u;
+  return e > 2u ? e - 2u : 0u;
+}
+
+// 2^(127 - s), the factor that brings a block into E2M1's range; 0 for a block
+// of NaN. s <= 252 otherwise, so the result is a normal number.
+__device__ __forceinline__ float MxInverseScale(uint32_t s) {
+  return s == 255u ? 0.0f : __uint_as_float((254u - s) << 23);
+}
+
+// 2^(s - 127), NaN for s = 255.
+__device__ __forceinline__ float MxScale(uint32_t s) {
+  if (s == 0u) return __uint_as_float(0x00400000u);
+  return s == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s << 23);
+}
+
+// Two E2M1 codes in one byte (lo in the low half): nearest, ties to even,
+// saturating at 6.
+__device__ __forceinline__ uint32_t MxCodes2(float lo, float hi) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "mov.b32 %0, {a, a, a, a};\n\t}"
+      : "=r"(r)
+      : "f"(lo), "f"(hi));
+  return r & 0xffu;
+}
+
+// Eight codes in one word, element 0 lowest.
+__device__ __forceinline__ uint32_t MxCodes8(const float (&v)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
+      : "=r"(r)
+      : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+        "f"(v[6]), "f"(v[7]));
+  return r;
+}
+
+// The value of the code in the low four bits: its exponent and fraction bits
+// placed at a float's (a subnormal there for the code 0.5) and rescaled.
+__device__ __forceinline__ float MxCodeValue(uint32_t code) {
+  const float m =
+      __uint_as_float(((code & 8u) << 28) | ((code & 7u) << 22));
+  return m * __uint_as_float(253u << 23);  // 2^126
+}
+
+// Byte offset of the scale of block b of (padded) row r.
+__device__ __forceinline__ int64_t MxScaleAt(int64_t r, int64_t b,
+                                             int64_t k_tiles) {
+  return ((r >> 7) * k_tiles + (b >> 2)) * kMxTileBytes + (r & 31) * 16 +
+         ((r >> 5) & 3) * 4 + (b & 3);
+}
+
+// The expert of a sorted row: the number of experts that end at or before it.
+// All lanes of a warp call it together with the same row.
+__device__ __forceinline__ int ExpertOfRow(const int32_t* offsets,
+                                           int num_experts, int row,
+                                           int lane) {
+  int e = 0;
+  for (int base = 0; base < num_experts; base += 32) {
+    const int i = base + lane;
+    const bool before = i < num_experts && __ldg(offsets + i + 1) <= row;
+    const unsigned ballot = __ballot_sync(0xffffffffu, before);
+    e += __popc(ballot);
+    if (ballot != 0xffffffffu) break;
+  }
+  return e;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace xse
+
+#endif  // XSE_MX_INTERNAL_H_
