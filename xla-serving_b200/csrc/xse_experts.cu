@@ -188,6 +188,7 @@ int LaunchSort(const void* ids, const xse_expert_plan& plan, cudaStream_t s) {
 // --------------------------------------------------------------- row movers
 
 constexpr int kThreads = 256;
+constexpr int kChoices = 8;  // a token's choices handled at a time
 
 // A piece of a row as a thread holds it: V elements, loaded and stored whole.
 template <typename T, int V>
@@ -242,75 +243,434 @@ struct MoveParams {
   const int32_t* slots;
   int64_t src_stride, y_stride, dst_stride;
   int64_t tokens, pairs;
+  uint32_t src_bytes, y_bytes, dst_bytes;  // the strides, where they fit
   int32_t topk, num_experts, cols;
+  int32_t row_shift;   // 2^row_shift threads share a token's row
+  int32_t quads;       // rows of slots and weights are whole 16-byte quads
 };
 
 // Zeros behind the last sorted row of a [pairs, cols] output.
-template <typename T>
-__device__ void ZeroTail(const MoveParams& p) {
+template <typename T, int V>
+__device__ __forceinline__ void ZeroTail(const MoveParams& p) {
   const int64_t kept = max(0, __ldg(p.offsets + p.num_experts));
-  const int64_t total = (p.pairs - kept) * p.cols;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-       i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t r = i / p.cols;
-    static_cast<T*>(p.dst)[(kept + r) * p.dst_stride + (i - r * p.cols)] =
-        Narrow<T>(0.0f);
+  Piece<T, V> zero;
+#pragma unroll
+  for (int k = 0; k < V; ++k) zero.v[k] = Narrow<T>(0.0f);
+  for (int64_t r = kept + blockIdx.x; r < p.pairs; r += gridDim.x) {
+    T* row = static_cast<T*>(p.dst) + r * p.dst_stride;
+    for (int c = threadIdx.x * V; c < p.cols; c += blockDim.x * V) {
+      StorePiece<T, V>(row + c, zero);
+    }
   }
 }
 
-// One (token, piece) per thread and step.
+// The sorted row of choice j of token t, -1 for none.
+__device__ __forceinline__ int32_t SlotOf(const MoveParams& p, int64_t t,
+                                          int j) {
+  if (j >= p.topk) return -1;
+  const int32_t slot = __ldg(p.slots + t * p.topk + j);
+  return slot < p.pairs ? slot : -1;
+}
+
+// The sorted rows of choices [first, first + kChoices) of token t, -1 for none.
+__device__ __forceinline__ void LoadSlots(const MoveParams& p, int64_t t,
+                                          int first, int32_t (&slot)[kChoices]) {
+#pragma unroll
+  for (int j = 0; j < kChoices; ++j) {
+    slot[j] = SlotOf(p, t, first + j);
+  }
+}
+
+// 2^row_shift threads per token, a piece each at a time: the row is read once
+// and stored for all its choices.
 template <typename T, int V>
 __global__ void __launch_bounds__(kThreads)
     GatherKernel(const __grid_constant__ MoveParams p) {
-  const int pieces = p.cols / V;
-  const int64_t total = p.tokens * pieces;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-       i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t t = i / pieces;
-    const int64_t c = (i - t * pieces) * V;
-    const Piece<T, V> r = LoadPiece<T, V>(static_cast<const T*>(p.src) +
-                                          t * p.src_stride + c);
-    for (int j = 0; j < p.topk; ++j) {
-      const int32_t slot = __ldg(p.slots + t * p.topk + j);
-      if (slot < 0 || slot >= p.pairs) continue;
-      StorePiece<T, V>(static_cast<T*>(p.dst) + slot * p.dst_stride + c, r);
+  const int per_block = kThreads >> p.row_shift;
+  const int mine = threadIdx.x >> p.row_shift;
+  const int lane = threadIdx.x & ((1 << p.row_shift) - 1);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * per_block + mine;
+       t < p.tokens; t += static_cast<int64_t>(gridDim.x) * per_block) {
+    const T* x = static_cast<const T*>(p.src) + t * p.src_stride;
+    for (int first = 0; first < p.topk; first += kChoices) {
+      int32_t slot[kChoices];
+      LoadSlots(p, t, first, slot);
+      for (int c = lane * V; c < p.cols; c += V << p.row_shift) {
+        const Piece<T, V> r = LoadPiece<T, V>(x + c);
+#pragma unroll
+        for (int j = 0; j < kChoices; ++j) {
+          if (slot[j] < 0) continue;
+          StorePiece<T, V>(
+              static_cast<T*>(p.dst) + slot[j] * p.dst_stride + c, r);
+        }
+      }
     }
   }
-  ZeroTail<T>(p);
+  ZeroTail<T, V>(p);
 }
 
-template <typename T, int V>
+// Rings. A thread copies its 16 bytes of up to kC choices' rows into slots of
+// its own in shared memory with cp.async, several steps ahead of the step it
+// adds up: about 190 KB of rows are in flight per SM without holding a
+// register, and no thread waits for another.
+constexpr int kRingThreads = 512;
+constexpr int kRingSlots = 24;  // 16-byte slots per thread
+constexpr int kRingBytes = kRingThreads * kRingSlots * 16;
+
+template <int kC>
+struct Ring {
+  static constexpr int kSteps = kRingSlots / kC < 8 ? kRingSlots / kC : 8;
+
+  // Slots are interleaved by thread: 16-byte accesses of a warp are contiguous.
+  __device__ static uint4* Slot(uint4* ring, int step, int j) {
+    return ring + (step * kC + j) * kRingThreads + threadIdx.x;
+  }
+  __device__ static void Copy(uint4* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                     static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+                 "l"(src)
+                 : "memory");
+  }
+  __device__ static void Commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  // All but the newest kSteps - 1 groups have landed.
+  __device__ static void Wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kSteps - 1) : "memory");
+  }
+};
+
+// Entries [first, first + kC) of token t's row of a [tokens, topk] array, as
+// quads where rows allow it; `none` past the last.
+template <int kC, typename E>
+__device__ __forceinline__ void LoadChoices(const MoveParams& p, const E* a,
+                                            int64_t t, int first, E none,
+                                            E (&v)[kC]) {
+  const E* row = a + t * p.topk + first;
+  if constexpr (kC >= 4) {
+    if (p.quads) {
+#pragma unroll
+      for (int j = 0; j < kC; j += 4) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        const bool there = first + j < p.topk;
+        if (there) u = __ldg(reinterpret_cast<const uint4*>(row + j));
+        __builtin_memcpy(&v[j], &u.x, 4);
+        __builtin_memcpy(&v[j + 1], &u.y, 4);
+        __builtin_memcpy(&v[j + 2], &u.z, 4);
+        __builtin_memcpy(&v[j + 3], &u.w, 4);
+        if (!there) v[j] = v[j + 1] = v[j + 2] = v[j + 3] = none;
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < kC; ++j) {
+    v[j] = first + j < p.topk ? __ldg(row + j) : none;
+  }
+}
+
+__device__ __forceinline__ bool Kept(const MoveParams& p, int32_t slot) {
+  return static_cast<uint32_t>(slot) < p.pairs;
+}
+
+// acc[k] += w * piece[k] in fp32, two at a time.
+__device__ __forceinline__ void Fma2(float2& acc, float2 a, float2 b) {
+  uint64_t c = reinterpret_cast<uint64_t&>(acc);
+  asm("fma.rn.f32x2 %0, %1, %2, %0;"
+      : "+l"(c)
+      : "l"(reinterpret_cast<uint64_t&>(a)),
+        "l"(reinterpret_cast<uint64_t&>(b)));
+  reinterpret_cast<uint64_t&>(acc) = c;
+}
+
+// A 16-byte piece widened to pairs of floats.
+template <typename T>
+struct Pairs {
+  static constexpr int kN = 8 / sizeof(T);
+  float2 v[kN];
+  __device__ explicit Pairs(const uint4& u) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = make_float2(__uint_as_float(w[i] << 16),
+                           __uint_as_float(w[i] & 0xffff0000u));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        v[i] = make_float2(__uint_as_float(w[2 * i]),
+                           __uint_as_float(w[2 * i + 1]));
+      }
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ uint4 NarrowPairs(const float2* v) {
+  Piece<T, 16 / sizeof(T)> o;
+#pragma unroll
+  for (int i = 0; i < Pairs<T>::kN; ++i) {
+    o.v[2 * i] = Narrow<T>(v[i].x);
+    o.v[2 * i + 1] = Narrow<T>(v[i].y);
+  }
+  uint4 u;
+  __builtin_memcpy(&u, &o, 16);
+  return u;
+}
+
+// The address of byte `at` of sorted row `slot` (rows closer than 4 GB).
+__device__ __forceinline__ const char* SortedRow(const void* base,
+                                                 uint32_t row_bytes,
+                                                 int32_t slot, uint32_t at) {
+  return static_cast<const char*>(base) +
+         static_cast<uint64_t>(static_cast<uint32_t>(slot)) * row_bytes + at;
+}
+
+// Steps of a thread: tokens, then pieces of the row, then groups of choices.
+// The slots of the next step to copy are loaded a step early.
+template <typename T, int kC>
+__global__ void __launch_bounds__(kRingThreads, 1)
+    CombineRingKernel(const __grid_constant__ MoveParams p) {
+  using R = Ring<kC>;
+  constexpr int kN = Pairs<T>::kN;
+  extern __shared__ uint4 ring[];
+  const int per_block = kRingThreads >> p.row_shift;
+  const uint32_t lane = (threadIdx.x & ((1 << p.row_shift) - 1)) * 16;
+  const uint32_t row_end = p.cols * static_cast<uint32_t>(sizeof(T));
+  const int64_t step_t = static_cast<int64_t>(gridDim.x) * per_block;
+  struct At {
+    int64_t t;
+    uint32_t byte;
+    int first;
+  };
+  const auto next = [&](At& at) {
+    at.first += kC;
+    if (at.first < p.topk) return;
+    at.first = 0;
+    at.byte += 16u << p.row_shift;
+    if (at.byte < row_end) return;
+    at.byte = lane;
+    at.t += step_t;
+  };
+  At tail{static_cast<int64_t>(blockIdx.x) * per_block +
+              (threadIdx.x >> p.row_shift),
+          lane, 0};
+  if (lane >= row_end) tail.t = p.tokens;
+  At head = tail;
+  int32_t ahead[kC];
+  if (head.t < p.tokens) {
+    LoadChoices<kC>(p, p.slots, head.t, head.first, -1, ahead);
+  }
+  int in = 0;
+  const auto issue = [&] {
+    if (head.t < p.tokens) {
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        if (Kept(p, ahead[j])) {
+          R::Copy(R::Slot(ring, in, j),
+                  SortedRow(p.src, p.src_bytes, ahead[j], head.byte));
+        }
+      }
+      next(head);
+      if (head.t < p.tokens) {
+        LoadChoices<kC>(p, p.slots, head.t, head.first, -1, ahead);
+      }
+    }
+    R::Commit();
+    in = in + 1 == R::kSteps ? 0 : in + 1;
+  };
+  for (int i = 0; i < R::kSteps - 1; ++i) issue();
+  float2 sum[kN];
+#pragma unroll
+  for (int k = 0; k < kN; ++k) sum[k] = make_float2(0.0f, 0.0f);
+  for (int out = 0; tail.t < p.tokens;
+       out = out + 1 == R::kSteps ? 0 : out + 1) {
+    issue();
+    int32_t slot[kC];
+    float w[kC];
+    LoadChoices<kC>(p, p.slots, tail.t, tail.first, -1, slot);
+    if (p.weights != nullptr) {
+      LoadChoices<kC>(p, p.weights, tail.t, tail.first, 0.0f, w);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kC; ++j) w[j] = 1.0f;
+    }
+    R::Wait();
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+      if (!Kept(p, slot[j])) continue;
+      const Pairs<T> r(*R::Slot(ring, out, j));
+#pragma unroll
+      for (int k = 0; k < kN; ++k) {
+        Fma2(sum[k], make_float2(w[j], w[j]), r.v[k]);
+      }
+    }
+    const At at = tail;
+    next(tail);
+    if (tail.first != 0) continue;
+    char* dst = static_cast<char*>(p.dst) +
+                at.t * p.dst_stride * static_cast<int64_t>(sizeof(T)) + at.byte;
+    __stcs(reinterpret_cast<uint4*>(dst), NarrowPairs<T>(sum));
+#pragma unroll
+    for (int k = 0; k < kN; ++k) sum[k] = make_float2(0.0f, 0.0f);
+  }
+}
+
+// Up to 32 threads per token, so that its dot products are added with
+// shuffles. Steps of a thread: tokens, then groups of choices, then pieces.
+// All threads of a block take the same steps.
+template <typename T, int kC>
+__global__ void __launch_bounds__(kRingThreads, 1)
+    CombineBackwardRingKernel(const __grid_constant__ MoveParams p) {
+  using R = Ring<kC>;
+  constexpr int kN = Pairs<T>::kN;
+  extern __shared__ uint4 ring[];
+  const int per_block = kRingThreads >> p.row_shift;
+  const uint32_t lane = (threadIdx.x & ((1 << p.row_shift) - 1)) * 16;
+  const uint32_t row_end = p.cols * static_cast<uint32_t>(sizeof(T));
+  const int64_t step_t = static_cast<int64_t>(gridDim.x) * per_block;
+  const int mine = threadIdx.x >> p.row_shift;
+  const bool dots = p.grad_weights != nullptr;
+  struct At {
+    int64_t t;  // of the block's first thread
+    int first;
+    uint32_t byte;
+  };
+  const auto next = [&](At& at) {
+    at.byte += 16u << p.row_shift;
+    if (at.byte < row_end) return;
+    at.byte = 0;
+    at.first += kC;
+    if (at.first < p.topk) return;
+    at.first = 0;
+    at.t += step_t;
+  };
+  const auto live = [&](const At& at) {
+    return at.t + mine < p.tokens && at.byte + lane < row_end;
+  };
+  const auto load = [&](const At& at, int32_t(&slot)[kC]) {
+    if (live(at)) {
+      LoadChoices<kC>(p, p.slots, at.t + mine, at.first, -1, slot);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kC; ++j) slot[j] = -1;
+    }
+  };
+  At tail{static_cast<int64_t>(blockIdx.x) * per_block, 0, 0};
+  At head = tail;
+  int32_t ahead[kC];
+  load(head, ahead);
+  int in = 0;
+  const auto issue = [&] {
+    if (dots && head.t < p.tokens) {
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        if (Kept(p, ahead[j])) {
+          R::Copy(R::Slot(ring, in, j),
+                  SortedRow(p.y, p.y_bytes, ahead[j], head.byte + lane));
+        }
+      }
+      next(head);
+      load(head, ahead);
+    }
+    R::Commit();
+    in = in + 1 == R::kSteps ? 0 : in + 1;
+  };
+  for (int i = 0; i < R::kSteps - 1; ++i) issue();
+  float2 dot[kC];
+#pragma unroll
+  for (int j = 0; j < kC; ++j) dot[j] = make_float2(0.0f, 0.0f);
+  for (int out = 0; tail.t < p.tokens;
+       out = out + 1 == R::kSteps ? 0 : out + 1) {
+    const int64_t t = tail.t + mine;
+    const bool here = live(tail);
+    uint4 g = make_uint4(0, 0, 0, 0);
+    if (here) {
+      g = __ldcs(reinterpret_cast<const uint4*>(
+          static_cast<const char*>(p.src) +
+          t * p.src_stride * static_cast<int64_t>(sizeof(T)) + tail.byte +
+          lane));
+    }
+    issue();
+    int32_t slot[kC];
+    load(tail, slot);
+    const Pairs<T> a(g);
+    if (p.dst != nullptr) {
+      float w[kC];
+#pragma unroll
+      for (int j = 0; j < kC; ++j) w[j] = 1.0f;
+      if (here && p.weights != nullptr) {
+        LoadChoices<kC>(p, p.weights, t, tail.first, 0.0f, w);
+      }
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        if (!Kept(p, slot[j])) continue;
+        float2 o[kN];
+#pragma unroll
+        for (int k = 0; k < kN; ++k) {
+          o[k] = make_float2(w[j] * a.v[k].x, w[j] * a.v[k].y);
+        }
+        __stcs(reinterpret_cast<uint4*>(const_cast<char*>(
+                   SortedRow(p.dst, p.dst_bytes, slot[j], tail.byte + lane))),
+               NarrowPairs<T>(o));
+      }
+    }
+    R::Wait();
+    if (dots) {
+#pragma unroll
+      for (int j = 0; j < kC; ++j) {
+        if (!Kept(p, slot[j])) continue;
+        const Pairs<T> b(*R::Slot(ring, out, j));
+#pragma unroll
+        for (int k = 0; k < kN; ++k) Fma2(dot[j], a.v[k], b.v[k]);
+      }
+    }
+    const At at = tail;
+    next(tail);
+    if (tail.byte != 0 || !dots) continue;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+      float sum = dot[j].x + dot[j].y;
+      for (int o = (1 << p.row_shift) >> 1; o >= 1; o >>= 1) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      }
+      if (lane == 0 && t < p.tokens && at.first + j < p.topk) {
+        p.grad_weights[t * p.topk + at.first + j] = sum;
+      }
+      dot[j] = make_float2(0.0f, 0.0f);
+    }
+  }
+  if (p.dst != nullptr) ZeroTail<T, 16 / sizeof(T)>(p);
+}
+
+// Rows at any alignment: one element at a time, several tokens per block.
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
     CombineKernel(const __grid_constant__ MoveParams p) {
-  const int pieces = p.cols / V;
-  const int64_t total = p.tokens * pieces;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-       i < total; i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t t = i / pieces;
-    const int64_t c = (i - t * pieces) * V;
-    float sum[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) sum[k] = 0.0f;
+  const int per_block = kThreads >> p.row_shift;
+  const int lane = threadIdx.x & ((1 << p.row_shift) - 1);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * per_block +
+                   (threadIdx.x >> p.row_shift);
+       t < p.tokens; t += static_cast<int64_t>(gridDim.x) * per_block) {
+    for (int c = lane; c < p.cols; c += 1 << p.row_shift) {
+      float sum = 0.0f;
 #pragma unroll 4
-    for (int j = 0; j < p.topk; ++j) {
-      const int32_t slot = __ldg(p.slots + t * p.topk + j);
-      if (slot < 0 || slot >= p.pairs) continue;
-      const float w = p.weights ? __ldg(p.weights + t * p.topk + j) : 1.0f;
-      const Piece<T, V> r = LoadPiece<T, V>(static_cast<const T*>(p.src) +
-                                            slot * p.src_stride + c);
-#pragma unroll
-      for (int k = 0; k < V; ++k) sum[k] = fmaf(w, Widen(r.v[k]), sum[k]);
+      for (int j = 0; j < p.topk; ++j) {
+        const int32_t slot = SlotOf(p, t, j);
+        if (slot < 0) continue;
+        const float w = p.weights ? __ldg(p.weights + t * p.topk + j) : 1.0f;
+        sum = fmaf(w, Widen(static_cast<const T*>(p.src)[slot * p.src_stride +
+                                                         c]), sum);
+      }
+      static_cast<T*>(p.dst)[t * p.dst_stride + c] = Narrow<T>(sum);
     }
-    Piece<T, V> out;
-#pragma unroll
-    for (int k = 0; k < V; ++k) out.v[k] = Narrow<T>(sum[k]);
-    StorePiece<T, V>(static_cast<T*>(p.dst) + t * p.dst_stride + c, out);
   }
 }
 
-// One warp per (token, choice): the gradient row scaled into its sorted row,
-// and its dot product with the expert's row.
-template <typename T, int V>
+// The same for the gradients: one warp per (token, choice).
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
     CombineBackwardKernel(const __grid_constant__ MoveParams p) {
   const int lane = threadIdx.x & 31;
@@ -318,28 +678,19 @@ __global__ void __launch_bounds__(kThreads)
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) +
                    threadIdx.x / 32;
        i < p.pairs; i += warps) {
-    const int32_t slot = __ldg(p.slots + i);
+    const int64_t t = i / p.topk;
+    const int32_t slot = SlotOf(p, t, static_cast<int>(i - t * p.topk));
     float dot = 0.0f;
-    if (slot >= 0 && slot < p.pairs) {
-      const T* g = static_cast<const T*>(p.src) + i / p.topk * p.src_stride;
+    if (slot >= 0) {
+      const T* g = static_cast<const T*>(p.src) + t * p.src_stride;
       const T* y = static_cast<const T*>(p.y) + slot * p.y_stride;
       T* d = static_cast<T*>(p.dst) + slot * p.dst_stride;
       const float w = p.weights ? __ldg(p.weights + i) : 1.0f;
-      for (int c = lane * V; c < p.cols; c += 32 * V) {
-        const Piece<T, V> a = LoadPiece<T, V>(g + c);
-        if (p.grad_weights != nullptr) {
-          const Piece<T, V> b = LoadPiece<T, V>(y + c);
-#pragma unroll
-          for (int k = 0; k < V; ++k) {
-            dot = fmaf(Widen(a.v[k]), Widen(b.v[k]), dot);
-          }
-        }
-        if (p.dst != nullptr) {
-          Piece<T, V> o;
-#pragma unroll
-          for (int k = 0; k < V; ++k) o.v[k] = Narrow<T>(w * Widen(a.v[k]));
-          StorePiece<T, V>(d + c, o);
-        }
+#pragma unroll 4
+      for (int c = lane; c < p.cols; c += 32) {
+        const float a = Widen(g[c]);
+        if (p.grad_weights != nullptr) dot = fmaf(a, Widen(y[c]), dot);
+        if (p.dst != nullptr) d[c] = Narrow<T>(w * a);
       }
     }
     if (p.grad_weights != nullptr) {
@@ -350,50 +701,93 @@ __global__ void __launch_bounds__(kThreads)
       if (lane == 0) p.grad_weights[i] = dot;
     }
   }
-  if (p.dst != nullptr) ZeroTail<T>(p);
-}
-
-int BlocksFor(int64_t work) {
-  const int64_t b = (work + kThreads - 1) / kThreads;
-  const int64_t most = static_cast<int64_t>(kNumSms) * 8;  // one wave
-  return static_cast<int>(b < 1 ? 1 : (b > most ? most : b));
+  if (p.dst != nullptr) ZeroTail<T, 1>(p);
 }
 
 enum : int { kGather, kCombine, kBackward };
 
-template <typename T, int V>
-void LaunchMove(int op, const MoveParams& p, cudaStream_t s) {
-  const int64_t pieces = p.tokens * (p.cols / V);
-  if (op == kGather) {
-    GatherKernel<T, V><<<BlocksFor(pieces), kThreads, 0, s>>>(p);
-  } else if (op == kCombine) {
-    CombineKernel<T, V><<<BlocksFor(pieces), kThreads, 0, s>>>(p);
-  } else {
-    CombineBackwardKernel<T, V>
-        <<<BlocksFor(p.pairs * 32), kThreads, 0, s>>>(p);
-  }
+// The smallest 2^n <= `most` threads with a piece each.
+int ThreadShift(int pieces, int most) {
+  int shift = 0;
+  while ((1 << shift) < pieces && (2 << shift) <= most) ++shift;
+  return shift;
+}
+
+int Blocks(int64_t work, int per_block, int per_sm) {
+  const int64_t need = (work + per_block - 1) / per_block;
+  const int64_t most = static_cast<int64_t>(kNumSms) * per_sm;  // one wave
+  return static_cast<int>(need < 1 ? 1 : need > most ? most : need);
+}
+
+template <typename T, int kC>
+cudaError_t LaunchRing(int op, MoveParams p, cudaStream_t s) {
+  const auto kernel = op == kCombine ? CombineRingKernel<T, kC>
+                                     : CombineBackwardRingKernel<T, kC>;
+  p.row_shift = ThreadShift(p.cols / (16 / static_cast<int>(sizeof(T))),
+                            op == kCombine ? 256 : 32);
+  const cudaError_t e = cudaFuncSetAttribute(
+      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  if (e != cudaSuccess) return e;
+  kernel<<<Blocks(p.tokens, kRingThreads >> p.row_shift, 1), kRingThreads,
+           kRingBytes, s>>>(p);
+  return cudaGetLastError();
 }
 
 template <typename T>
-void LaunchMoveAs(int op, const MoveParams& p, cudaStream_t s) {
+cudaError_t LaunchMove(int op, MoveParams p, bool vec, cudaStream_t s) {
   constexpr int kV = 16 / sizeof(T);
+  if (op == kGather) {
+    p.row_shift = ThreadShift(vec ? p.cols / kV : p.cols, kThreads);
+    const int blocks = Blocks(p.tokens, kThreads >> p.row_shift, 8);
+    if (vec) {
+      GatherKernel<T, kV><<<blocks, kThreads, 0, s>>>(p);
+    } else {
+      GatherKernel<T, 1><<<blocks, kThreads, 0, s>>>(p);
+    }
+  } else if (vec) {
+    return p.topk == 1   ? LaunchRing<T, 1>(op, p, s)
+           : p.topk == 2 ? LaunchRing<T, 2>(op, p, s)
+           : p.topk <= 4 ? LaunchRing<T, 4>(op, p, s)
+                         : LaunchRing<T, 8>(op, p, s);
+  } else if (op == kCombine) {
+    p.row_shift = ThreadShift(p.cols, kThreads);
+    CombineKernel<T><<<Blocks(p.tokens, kThreads >> p.row_shift, 8), kThreads,
+                       0, s>>>(p);
+  } else {
+    CombineBackwardKernel<T>
+        <<<Blocks(p.pairs, kThreads / 32, 8), kThreads, 0, s>>>(p);
+  }
+  return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t LaunchMoveAs(int op, MoveParams p, cudaStream_t s) {
+  constexpr int kV = 16 / sizeof(T);
+  constexpr int64_t kMost = (int64_t{1} << 32) / sizeof(T);
   const bool vec = p.cols % kV == 0 && Aligned16(p.src) && Aligned16(p.y) &&
                    Aligned16(p.dst) && p.src_stride % kV == 0 &&
-                   p.y_stride % kV == 0 && p.dst_stride % kV == 0;
-  if (vec) {
-    LaunchMove<T, kV>(op, p, s);
-  } else {
-    LaunchMove<T, 1>(op, p, s);
-  }
+                   p.y_stride % kV == 0 && p.dst_stride % kV == 0 &&
+                   p.src_stride < kMost && p.y_stride < kMost &&
+                   p.dst_stride < kMost;
+  p.src_bytes = static_cast<uint32_t>(p.src_stride * sizeof(T));
+  p.y_bytes = static_cast<uint32_t>(p.y_stride * sizeof(T));
+  p.dst_bytes = static_cast<uint32_t>(p.dst_stride * sizeof(T));
+  p.quads = p.topk % 4 == 0 && Aligned16(p.slots) && Aligned16(p.weights);
+  return LaunchMove<T>(op, p, vec, s);
 }
 
 int RunMove(int op, int32_t dtype, const MoveParams& p, const char* what,
             cudaStream_t s) {
-  if (dtype == XSE_DT_F32) LaunchMoveAs<float>(op, p, s);
-  if (dtype == XSE_DT_BF16) LaunchMoveAs<__nv_bfloat16>(op, p, s);
-  const int rc = LaunchStatus(what);
-  if (rc == XSE_OK) SetLastLaunchCount(1);
-  return rc;
+  const cudaError_t e = dtype == XSE_DT_F32
+                            ? LaunchMoveAs<float>(op, p, s)
+                            : LaunchMoveAs<__nv_bfloat16>(op, p, s);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return FailWith(XSE_INTERNAL, "%s launch: %s", what,
+                    cudaGetErrorString(e));
+  }
+  SetLastLaunchCount(1);
+  return XSE_OK;
 }
 
 int CheckRows(const xse_expert_plan* plan, int32_t dtype, int32_t cols) {

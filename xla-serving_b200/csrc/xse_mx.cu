@@ -61,8 +61,39 @@ int CheckMxMatrix(const xse_mx_matrix* q, const char* what) {
 
 namespace {
 
-constexpr int kThreads = 128;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 256;
+constexpr int kWarpShift = 3;  // warps of a block
+
+// The rows of a kernel whose warps take `chunks` pieces of a row each in turn:
+// 2^row_shift warps a row, so that no index needs a division.
+int RowShift(int64_t chunks) {
+  int shift = 0;
+  while (shift < kWarpShift && (1 << shift) < chunks) ++shift;
+  return shift;
+}
+
+int BlocksForRows(int64_t rows, int row_shift) {
+  const int64_t per = 1 << (kWarpShift - row_shift);
+  const int64_t b = (rows + per - 1) / per;
+  const int64_t most = static_cast<int64_t>(kNumSms) * 8;  // one wave
+  return static_cast<int>(b > most ? most : b);
+}
+
+struct WarpRow {
+  int64_t row, step;  // first row of this warp, rows of a step
+  int chunk, chunks;  // first piece of the row, pieces of a step
+};
+
+__device__ __forceinline__ WarpRow FirstRow(int row_shift) {
+  const int warp = threadIdx.x / 32;
+  WarpRow w;
+  w.chunks = 1 << row_shift;
+  w.chunk = warp & (w.chunks - 1);
+  const int per = 1 << (kWarpShift - row_shift);
+  w.row = static_cast<int64_t>(blockIdx.x) * per + (warp >> row_shift);
+  w.step = static_cast<int64_t>(gridDim.x) * per;
+  return w;
+}
 
 // Where quantised rows go: row r of group g to code row g * rows + r, or (with
 // a plan) token row t to the sorted rows of its choices, or sorted row r to
@@ -74,6 +105,8 @@ struct QuantParams {
   int64_t group_stride, row_stride, col_stride;
   int64_t rows;         // of a group
   int64_t total_rows;   // groups * rows
+  int32_t groups;
+  int32_t row_shift;    // 2^row_shift warps share a row
   int32_t cols;
   int32_t k_tiles;
   int64_t row_bytes;
@@ -116,7 +149,7 @@ __device__ __forceinline__ void Load8(const __nv_bfloat16* p, float (&v)[8]) {
 
 template <typename T>
 __device__ __forceinline__ const T* RowOf(const QuantParams& p, int64_t row) {
-  const int64_t g = row / p.rows;
+  const int64_t g = p.groups == 1 ? 0 : row / p.rows;
   return static_cast<const T*>(p.x) + g * p.group_stride +
          (row - g * p.rows) * p.row_stride;
 }
@@ -126,7 +159,7 @@ template <int kMode, typename Put>
 __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
                                           int lane, Put put) {
   if constexpr (kMode == kPlain) {
-    const int64_t g = row / p.rows;
+    const int64_t g = p.groups == 1 ? 0 : row / p.rows;
     put(row, g * p.row_tiles * kMxTileRows + (row - g * p.rows));
   } else {
     const int count = kMode == kFromTokens ? p.topk : 1;
@@ -140,118 +173,139 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
       const int32_t begin = __ldg(p.offsets + e);
       if (begin < 0 || begin > slot) continue;
       const int local = slot - begin;
-      const int64_t tile = begin / p.tile_rows + e + local / p.tile_rows;
+      const int in_tile = local % p.tile_rows;
+      const int64_t tile =
+          (begin / p.tile_rows + e + local / p.tile_rows) *
+              (p.tile_rows > kMxTileRows ? 2 : 1) + in_tile / kMxTileRows;
       if (tile >= p.row_tiles) continue;
       put(static_cast<int64_t>(slot),
-          tile * kMxTileRows + local % p.tile_rows);
+          tile * kMxTileRows + in_tile % kMxTileRows);
     }
   }
 }
 
-// A warp takes 256 columns of a row, a lane 8 of them; four lanes share a
+// A warp takes 512 columns of a row, a lane 8 of each half; four lanes share a
 // block and agree on its largest magnitude with two shuffles.
 template <typename T, int kMode>
 __global__ void __launch_bounds__(kThreads)
     QuantizeVecKernel(const __grid_constant__ QuantParams p) {
   const int lane = threadIdx.x & 31;
-  const int chunks = (p.k_tiles + 1) / 2;
-  const int64_t units = p.total_rows * chunks;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-       u < units; u += step) {
-    const int64_t row = u / chunks;
-    const int col = static_cast<int>(u - row * chunks) * 256 + lane * 8;
-    const T* x = RowOf<T>(p, row) + col;
-    float v[8];
-    if (col + 8 <= p.cols) {
-      Load8(x, v);
-    } else {
+  const int padded = p.k_tiles * 128, code_cols = (p.cols + 31) / 32 * 32;
+  const WarpRow w = FirstRow(p.row_shift);
+  for (int64_t row = w.row; row < p.total_rows; row += w.step) {
+    const T* x = RowOf<T>(p, row);
+    for (int first = w.chunk * 512; first < padded; first += w.chunks * 512) {
+      float v[2][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        v[i] = col + i < p.cols ? ToFloat(x[i]) : 0.0f;
+      for (int h = 0; h < 2; ++h) {
+        const int col = first + h * 256 + lane * 8;
+        if (col + 8 <= p.cols) {
+          Load8(x + col, v[h]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            v[h][i] = col + i < p.cols ? ToFloat(x[col + i]) : 0.0f;
+          }
+        }
       }
+      uint32_t word[2], scales[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          most = max(most, __float_as_uint(v[h][i]) & 0x7fffffffu);
+        }
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        const uint32_t s = MxScaleByte(most);
+        const float inv = MxInverseScale(s);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[h][i] *= inv;
+        word[h] = s == 255u ? 0u : MxCodes8(v[h]);
+        // The scale bytes of four blocks (16 lanes) as one word.
+        scales[h] = s | __shfl_down_sync(0xffffffffu, s, 4) << 8;
+        scales[h] |= __shfl_down_sync(0xffffffffu, scales[h], 8) << 16;
+      }
+      ForPlaces<kMode>(p, row, lane, [&](int64_t code_row, int64_t scale_row) {
+        uint8_t* codes = p.codes + code_row * p.row_bytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int col = first + h * 256 + lane * 8;
+          if (col < code_cols) {
+            *reinterpret_cast<uint32_t*>(codes + col / 2) = word[h];
+          }
+          if ((lane & 15) == 0 && col < padded) {
+            *reinterpret_cast<uint32_t*>(
+                p.scales + MxScaleAt(scale_row, col / 32, p.k_tiles)) =
+                scales[h];
+          }
+        }
+      });
     }
-    uint32_t most = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      most = max(most, __float_as_uint(v[i]) & 0x7fffffffu);
-    }
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const uint32_t s = MxScaleByte(most);
-    const float inv = MxInverseScale(s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= inv;
-    const uint32_t word = s == 255u ? 0u : MxCodes8(v);
-    // The scale bytes of four blocks (16 lanes) as one word.
-    uint32_t scales = s | __shfl_down_sync(0xffffffffu, s, 4) << 8;
-    scales |= __shfl_down_sync(0xffffffffu, scales, 8) << 16;
-    const bool has_codes = col < (p.cols + 31) / 32 * 32;
-    const bool has_scales = (lane & 15) == 0 && col < p.k_tiles * 128;
-    ForPlaces<kMode>(p, row, lane, [&](int64_t code_row, int64_t scale_row) {
-      if (has_codes) {
-        *reinterpret_cast<uint32_t*>(p.codes + code_row * p.row_bytes +
-                                     col / 2) = word;
-      }
-      if (has_scales) {
-        *reinterpret_cast<uint32_t*>(
-            p.scales + MxScaleAt(scale_row, col / 32, p.k_tiles)) = scales;
-      }
-    });
   }
 }
 
-// A warp takes 128 columns of a row as four blocks of 32 lanes. Lane l ends
-// with the word of block 2 (l & 1) + (l >> 1 & 1), bytes 4 (l >> 3) on.
+// A warp takes 256 columns of a row as two halves of four blocks of 32 lanes.
+// Lane l ends with the word of block 2 (l & 1) + (l >> 1 & 1) of each half,
+// bytes 4 (l >> 3) on.
 template <typename T, int kMode>
 __global__ void __launch_bounds__(kThreads)
     QuantizeWarpKernel(const __grid_constant__ QuantParams p) {
   const unsigned all = 0xffffffffu;
   const int lane = threadIdx.x & 31;
-  const int64_t units = p.total_rows * p.k_tiles;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-       u < units; u += step) {
-    const int64_t row = u / p.k_tiles;
-    const int first = static_cast<int>(u - row * p.k_tiles) * 128;
+  const bool odd = lane & 1, odd2 = lane & 2;
+  const int padded = p.k_tiles * 128, code_cols = (p.cols + 31) / 32 * 32;
+  const WarpRow w = FirstRow(p.row_shift);
+  for (int64_t row = w.row; row < p.total_rows; row += w.step) {
     const T* x = RowOf<T>(p, row);
-    float v[4];
+    for (int first = w.chunk * 256; first < padded; first += w.chunks * 256) {
+      float v[8];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int col = first + 32 * b + lane;
-      v[b] = col < p.cols ? ToFloat(x[col]) : 0.0f;
-    }
-    uint32_t scales = 0;
+      for (int b = 0; b < 8; ++b) {
+        const int col = first + 32 * b + lane;
+        v[b] = col < p.cols ? ToFloat(x[col]) : 0.0f;
+      }
+      uint32_t word[2], scales[2];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const uint32_t s = MxScaleByte(
-          __reduce_max_sync(all, __float_as_uint(v[b]) & 0x7fffffffu));
-      scales |= s << (8 * b);
-      v[b] = s == 255u ? 0.0f : v[b] * MxInverseScale(s);
+      for (int h = 0; h < 2; ++h) {
+        float* u = v + 4 * h;
+        scales[h] = 0;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t s = MxScaleByte(
+              __reduce_max_sync(all, __float_as_uint(u[b]) & 0x7fffffffu));
+          scales[h] |= s << (8 * b);
+          u[b] = s == 255u ? 0.0f : u[b] * MxInverseScale(s);
+        }
+        // Even lanes keep blocks 0 and 1, odd lanes 2 and 3, of a pair of
+        // elements; then each lane one block of two pairs; then of four.
+        const float r0 = __shfl_xor_sync(all, odd ? u[0] : u[2], 1);
+        const float r1 = __shfl_xor_sync(all, odd ? u[1] : u[3], 1);
+        const uint32_t b0 = odd ? MxCodes2(r0, u[2]) : MxCodes2(u[0], r0);
+        const uint32_t b1 = odd ? MxCodes2(r1, u[3]) : MxCodes2(u[1], r1);
+        const uint32_t got = __shfl_xor_sync(all, odd2 ? b0 : b1, 2);
+        word[h] = odd2 ? (got | b1 << 8) : (b0 | got << 8);
+        word[h] |= __shfl_down_sync(all, word[h], 4) << 16;
+      }
+      const int block = (odd ? 2 : 0) + (odd2 ? 1 : 0);
+      ForPlaces<kMode>(p, row, lane, [&](int64_t code_row, int64_t scale_row) {
+        uint8_t* codes = p.codes + code_row * p.row_bytes;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int half = first + 128 * h;
+          const int col = half + 32 * block + 8 * (lane >> 3);
+          if ((lane & 4) == 0 && col < code_cols) {
+            *reinterpret_cast<uint32_t*>(codes + col / 2) = word[h];
+          }
+          if (lane == 0 && half < padded) {
+            *reinterpret_cast<uint32_t*>(
+                p.scales + MxScaleAt(scale_row, half / 32, p.k_tiles)) =
+                scales[h];
+          }
+        }
+      });
     }
-    // Even lanes keep blocks 0 and 1, odd lanes 2 and 3, of a pair of
-    // elements; then each lane one block of two pairs; then of four.
-    const bool odd = lane & 1, odd2 = lane & 2;
-    const float r0 = __shfl_xor_sync(all, odd ? v[0] : v[2], 1);
-    const float r1 = __shfl_xor_sync(all, odd ? v[1] : v[3], 1);
-    const uint32_t b0 = odd ? MxCodes2(r0, v[2]) : MxCodes2(v[0], r0);
-    const uint32_t b1 = odd ? MxCodes2(r1, v[3]) : MxCodes2(v[1], r1);
-    const uint32_t got = __shfl_xor_sync(all, odd2 ? b0 : b1, 2);
-    uint32_t word = odd2 ? (got | b1 << 8) : (b0 | got << 8);
-    word |= __shfl_down_sync(all, word, 4) << 16;
-    const int col = first + 32 * ((odd ? 2 : 0) + (odd2 ? 1 : 0)) +
-                    8 * (lane >> 3);
-    const bool has_codes = (lane & 4) == 0 && col < (p.cols + 31) / 32 * 32;
-    ForPlaces<kMode>(p, row, lane, [&](int64_t code_row, int64_t scale_row) {
-      if (has_codes) {
-        *reinterpret_cast<uint32_t*>(p.codes + code_row * p.row_bytes +
-                                     col / 2) = word;
-      }
-      if (lane == 0) {
-        *reinterpret_cast<uint32_t*>(
-            p.scales + MxScaleAt(scale_row, first / 32, p.k_tiles)) = scales;
-      }
-    });
   }
 }
 
@@ -295,60 +349,65 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// A warp takes 128 columns of a row: 16 lanes load a word of eight codes each,
-// and every lane takes its element's word by a shuffle, so that the stores are
-// coalesced at any alignment.
+// A warp takes 256 columns of a row: its lanes load a word of eight codes
+// each, and every lane takes its element's word by a shuffle, so that the
+// stores are coalesced at any alignment.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     DequantizeKernel(const uint8_t* __restrict__ codes,
                      const uint8_t* __restrict__ scales, int64_t rows,
-                     int64_t total_rows, int cols, int64_t row_bytes,
-                     int k_tiles, int64_t row_tiles, T* __restrict__ out,
+                     int groups, int cols, int64_t row_bytes, int k_tiles,
+                     int64_t row_tiles, int row_shift, T* __restrict__ out,
                      int64_t group_stride, int64_t row_stride) {
   const int lane = threadIdx.x & 31;
-  const int64_t units = total_rows * k_tiles;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kWarps;
-  for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + threadIdx.x / 32;
-       u < units; u += step) {
-    const int64_t row = u / k_tiles;
-    const int first = static_cast<int>(u - row * k_tiles) * 128;
-    const int64_t g = row / rows;
+  const int padded = k_tiles * 128;
+  const WarpRow w = FirstRow(row_shift);
+  for (int64_t row = w.row; row < rows * groups; row += w.step) {
+    const int64_t g = groups == 1 ? 0 : row / rows;
     const int64_t r = row - g * rows;
-    uint32_t word = 0;
-    if (lane < 16 && first / 2 + lane * 4 < row_bytes) {
-      word = __ldg(reinterpret_cast<const uint32_t*>(
-          codes + row * row_bytes + first / 2 + lane * 4));
-    }
-    const uint32_t sc = __ldg(reinterpret_cast<const uint32_t*>(
-        scales + MxScaleAt(g * row_tiles * kMxTileRows + r, first / 32,
-                           k_tiles)));
     T* o = out + g * group_stride + r * row_stride;
+    for (int first = w.chunk * 256; first < padded; first += w.chunks * 256) {
+      const int at = first / 2 + lane * 4;
+      const uint32_t word =
+          at < row_bytes
+              ? __ldg(reinterpret_cast<const uint32_t*>(codes +
+                                                        row * row_bytes + at))
+              : 0u;
+      uint32_t sc[2];
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const uint32_t w = __shfl_sync(0xffffffffu, word, 4 * b + (lane >> 3));
-      const int col = first + 32 * b + lane;
-      const float v = MxCodeValue(w >> (4 * (lane & 7))) *
-                      MxScale(sc >> (8 * b) & 0xffu);
-      if (col < cols) o[col] = static_cast<T>(v);
+      for (int h = 0; h < 2; ++h) {
+        sc[h] = first + 128 * h < padded
+                    ? __ldg(reinterpret_cast<const uint32_t*>(
+                          scales + MxScaleAt(g * row_tiles * kMxTileRows + r,
+                                             first / 32 + 4 * h, k_tiles)))
+                    : 0u;
+      }
+#pragma unroll
+      for (int b = 0; b < 8; ++b) {
+        const uint32_t u = __shfl_sync(0xffffffffu, word, 4 * b + (lane >> 3));
+        const int col = first + 32 * b + lane;
+        const float v = MxCodeValue(u >> (4 * (lane & 7))) *
+                        MxScale(sc[b >> 2] >> (8 * (b & 3)) & 0xffu);
+        if (col < cols) o[col] = static_cast<T>(v);
+      }
     }
   }
 }
 
 int BlocksFor(int64_t work, int per_block) {
   const int64_t b = (work + per_block - 1) / per_block;
-  const int64_t most = static_cast<int64_t>(kNumSms) * 16;  // one wave
+  const int64_t most = static_cast<int64_t>(kNumSms) * 8;  // one wave
   return static_cast<int>(b < 1 ? 1 : (b > most ? most : b));
 }
 
 template <typename T, int kMode>
-void LaunchQuantize(const QuantParams& p, bool vec, cudaStream_t s) {
+void LaunchQuantize(QuantParams p, bool vec, cudaStream_t s) {
+  p.row_shift = RowShift(vec ? (p.k_tiles + 3) / 4 : (p.k_tiles + 1) / 2);
+  const int blocks = BlocksForRows(p.total_rows, p.row_shift);
   if (vec) {
-    QuantizeVecKernel<T, kMode>
-        <<<BlocksFor(p.total_rows * ((p.k_tiles + 1) / 2), kWarps), kThreads,
-           0, s>>>(p);
+    QuantizeVecKernel<T, kMode><<<blocks, kThreads, 0, s>>>(p);
   } else {
-    QuantizeWarpKernel<T, kMode>
-        <<<BlocksFor(p.total_rows * p.k_tiles, kWarps), kThreads, 0, s>>>(p);
+    QuantizeWarpKernel<T, kMode><<<blocks, kThreads, 0, s>>>(p);
   }
 }
 
@@ -385,6 +444,7 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
   p.row_stride = row_stride;
   p.col_stride = 1;
   p.rows = p.total_rows = rows;
+  p.groups = 1;
   p.cols = cols;
   p.k_tiles = static_cast<int32_t>(MxKTiles(cols));
   p.row_bytes = MxRowBytes(cols);
@@ -439,6 +499,7 @@ int xse_mxfp4_quantize(const void* x, int32_t dtype, int64_t group_stride,
   p.col_stride = q->cols == 1 ? 1 : col_stride;
   p.rows = q->rows;
   p.total_rows = q->rows * q->groups;
+  p.groups = q->groups;
   p.cols = q->cols;
   p.k_tiles = static_cast<int32_t>(MxKTiles(q->cols));
   p.row_bytes = MxRowBytes(q->cols);
@@ -471,21 +532,21 @@ int xse_mxfp4_dequantize(const xse_mx_matrix* q, void* out, int32_t dtype,
     return FailWith(XSE_INVALID_ARGUMENT, "4-bit values: out is null.");
   }
   const int k_tiles = static_cast<int>(MxKTiles(q->cols));
-  const int64_t total = q->rows * q->groups;
-  const int blocks = BlocksFor(total * k_tiles, kWarps);
+  const int row_shift = RowShift((k_tiles + 1) / 2);
+  const int blocks = BlocksForRows(q->rows * q->groups, row_shift);
   const uint8_t* codes = static_cast<const uint8_t*>(q->codes);
   const uint8_t* scales = static_cast<const uint8_t*>(q->scales);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == XSE_DT_F32) {
     DequantizeKernel<float><<<blocks, kThreads, 0, s>>>(
-        codes, scales, q->rows, total, q->cols, MxRowBytes(q->cols), k_tiles,
-        MxRowTiles(q->rows), static_cast<float*>(out), group_stride,
-        row_stride);
+        codes, scales, q->rows, q->groups, q->cols, MxRowBytes(q->cols),
+        k_tiles, MxRowTiles(q->rows), row_shift, static_cast<float*>(out),
+        group_stride, row_stride);
   } else {
     DequantizeKernel<__nv_bfloat16><<<blocks, kThreads, 0, s>>>(
-        codes, scales, q->rows, total, q->cols, MxRowBytes(q->cols), k_tiles,
-        MxRowTiles(q->rows), static_cast<__nv_bfloat16*>(out), group_stride,
-        row_stride);
+        codes, scales, q->rows, q->groups, q->cols, MxRowBytes(q->cols),
+        k_tiles, MxRowTiles(q->rows), row_shift,
+        static_cast<__nv_bfloat16*>(out), group_stride, row_stride);
   }
   const int rc = LaunchStatus("4-bit dequantisation");
   if (rc == XSE_OK) SetLastLaunchCount(1);

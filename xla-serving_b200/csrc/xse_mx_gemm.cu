@@ -16,7 +16,7 @@
 // One block per SM runs over its tiles: warp 0 copies stages of 256 elements
 // of k with TMA (codes, 128-byte swizzled; scales, 512-byte tiles as they lie
 // in memory), warp 1 moves the scales to tensor memory and issues the MMAs,
-// warps 2 to 5 write the previous tile's results from the second accumulator.
+// warps 2 to 9 write the results, which overlaps with the next tile's MMAs.
 //
 // Few tiles: a cluster of `split` blocks shares a tile, each taking a part of
 // k; the parts are added in block order over distributed shared memory.
@@ -37,8 +37,8 @@ namespace {
 
 constexpr int kM = 128;            // features of a tile
 constexpr int kStageK = 256;       // elements of k per stage (128 bytes)
-constexpr int kThreads = 192;
-constexpr int kEpilogueWarps = 4;
+constexpr int kEpilogueWarps = 8;  // two per quarter of the lanes
+constexpr int kThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kABytes = kM * kStageK / 2;
 constexpr int kScaleBytes = 2 * kMxTileBytes;  // a tile row's, per stage
 constexpr long long kWaitCycles = 4000000000ll;  // about two seconds
@@ -57,6 +57,9 @@ struct Config {
   static constexpr int kAccColumns = kN < 32 ? 32 : kN;
   static constexpr int kAccs = kN <= 192 ? 2 : 1;
   static constexpr int kScaleColumns = 8 * (1 + kBTiles);
+  // Columns that an epilogue warp takes (with 16 rows the second warp of a
+  // quarter has none).
+  static constexpr int kPart = kN < 32 ? 16 : kN / 2;
   static_assert(kAccs * kAccColumns + kStages * kScaleColumns <= 512,
                 "tensor memory");
 };
@@ -79,7 +82,7 @@ struct GemmParams {
   int32_t k_stages;
   int32_t m_tiles;
   int32_t activation;
-  int32_t y_bf16;
+  int32_t paired;          // bf16 y: 4-byte aligned pairs of features
   int32_t split;           // blocks of a cluster that share a tile's k
 };
 
@@ -87,6 +90,19 @@ struct GemmParams {
 
 __device__ __forceinline__ uint32_t SharedAddress(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// True in one lane of a converged warp. The compiler knows it to be one, so
+// the operands of what that lane issues stay in uniform registers (8192 x 8192
+// x 8192: 394 us with a test of the lane's index, 256 us with this).
+__device__ __forceinline__ bool Elect() {
+  uint32_t one;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one != 0;
 }
 
 __device__ __forceinline__ void BarrierInit(uint32_t bar, uint32_t count) {
@@ -195,11 +211,8 @@ __device__ __forceinline__ void Mma(uint32_t acc, uint64_t a, uint64_t b,
       : "memory");
 }
 
-template <int kColumns>
-__device__ __forceinline__ void LoadColumns(uint32_t address,
-                                            float (&v)[kColumns]) {
-  static_assert(kColumns == 16, "one instruction");
-  uint32_t r[16];
+// 16 columns of the calling warp's 32 lanes; complete after WaitLoads.
+__device__ __forceinline__ void LoadColumns(uint32_t address, uint32_t* r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, "
       "%8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -208,9 +221,10 @@ __device__ __forceinline__ void LoadColumns(uint32_t address,
         "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(address)
       : "memory");
+}
+
+__device__ __forceinline__ void WaitLoads() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 __device__ __forceinline__ void ClusterSync() {
@@ -292,7 +306,7 @@ __device__ __forceinline__ Tile TileOf(const GemmParams& p, int64_t item,
   t.row = first + at * kN;
   const int64_t left = count - at * kN;
   t.rows = static_cast<int>(left < kN ? left : kN);
-  t.b_tile = first / kN + t.group + at * C::kBTiles;
+  t.b_tile = (first / kN + t.group + at) * C::kBTiles;
   return t;
 }
 
@@ -302,17 +316,56 @@ __device__ __forceinline__ float Activate(float v, int activation) {
   return v;
 }
 
-__device__ __forceinline__ void StoreY(const GemmParams& p, int64_t row,
-                                       int feature, float v) {
-  if (p.y_bf16) {
-    static_cast<__nv_bfloat16*>(p.y)[row * p.y_stride + feature] =
-        __float2bfloat16_rn(v);
-  } else {
-    static_cast<float*>(p.y)[row * p.y_stride + feature] = v;
+__device__ __forceinline__ void Store(float* p, float v) { *p = v; }
+__device__ __forceinline__ void Store(__nv_bfloat16* p, float v) {
+  *p = __float2bfloat16_rn(v);
+}
+
+// 16 rows of y from the lane's accumulator columns: lane l holds feature l of
+// every row. `y` points at the first row's element of this lane; `rows` of the
+// 16 exist; `mine`: the feature does.
+template <typename T>
+__device__ __forceinline__ void StoreRows(T* y, int64_t stride,
+                                          const uint32_t* r, float bias,
+                                          int activation, int rows, bool mine,
+                                          bool paired, int lane) {
+  float v[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]) + bias;
+  if (activation == XSE_ACT_RELU) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = v[i] < 0.0f ? 0.0f : v[i];
+  } else if (activation == XSE_ACT_SIGMOID) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = Activate(v[i], XSE_ACT_SIGMOID);
+  }
+  if constexpr (sizeof(T) == 2) {
+    // Two features a store: even lanes take the even rows of a pair of lanes,
+    // odd lanes the odd ones.
+    if (paired) {
+      const bool odd = lane & 1;
+      y += odd ? stride - 1 : 0;
+      rows -= odd ? 1 : 0;
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        const float got =
+            __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
+        const float lo = odd ? got : v[i], hi = odd ? v[i + 1] : got;
+        if (mine && i < rows) {
+          *reinterpret_cast<__nv_bfloat162*>(y + i * stride) =
+              __floats2bfloat162_rn(lo, hi);
+        }
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    if (mine && i < rows) Store(y + i * stride, v[i]);
   }
 }
 
-template <int kN>
+template <int kN, typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     MxGemmKernel(const __grid_constant__ GemmParams p) {
   using C = Config<kN>;
@@ -329,7 +382,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* tile_begin =
       reinterpret_cast<int*>(stages + C::kStages * C::kStageBytes);
   int* row_begin = tile_begin + (p.groups + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % p.split;
 
   if (threadIdx.x == 0) {
@@ -394,25 +448,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t stage_base = SharedAddress(stages);
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      int64_t issued = 0;
-      for (int64_t item = first_item; ok && item < items; item += item_step) {
-        const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
-        const uint8_t* a_scales =
-            p.a_scales + (static_cast<int64_t>(t.group) * p.m_tiles + t.m) *
-                             p.k_tiles * kMxTileBytes;
-        const uint8_t* b_scales =
-            p.b_scales + t.b_tile * p.k_tiles * kMxTileBytes;
-        const bool b_first = t.b_tile < p.b_tiles;
-        const bool b_second = C::kBTiles == 2 && t.b_tile + 1 < p.b_tiles;
-        for (int s = k_begin; s < k_end; ++s) {
+    // The whole warp follows the loop; one lane issues.
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int64_t issued = 0;
+    for (int64_t item = first_item; ok && item < items; item += item_step) {
+      const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+      const uint8_t* a_scales =
+          p.a_scales + (static_cast<int64_t>(t.group) * p.m_tiles + t.m) *
+                           p.k_tiles * kMxTileBytes;
+      const uint8_t* b_scales =
+          p.b_scales + t.b_tile * p.k_tiles * kMxTileBytes;
+      const bool b_first = t.b_tile < p.b_tiles;
+      const bool b_second = C::kBTiles == 2 && t.b_tile + 1 < p.b_tiles;
+      for (int s = k_begin; s < k_end; ++s) {
+        ok = BarrierWait(SharedAddress(empty_bar + stage), phase ^ 1, &failed);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (Elect()) {
           const uint32_t bar = SharedAddress(full_bar + stage);
-          ok = BarrierWait(SharedAddress(empty_bar + stage), phase ^ 1,
-                           &failed);
-          if (!ok) break;
           const uint32_t at = stage_base + stage * C::kStageBytes;
           const uint32_t scales = at + kABytes + C::kBBytes;
           const uint32_t bytes =
@@ -431,127 +486,118 @@ __global__ void __launch_bounds__(kThreads, 1)
             BulkLoad(scales + 2 * kScaleBytes,
                      b_scales + p.k_tiles * kMxTileBytes + k_at, bytes, bar);
           }
-          ++issued;
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
-      }
-      // After a failure the copies in flight still have to land.
-      if (!ok) {
-        volatile int ignored = 0;
-        const int in_flight =
-            static_cast<int>(issued < C::kStages ? issued : C::kStages);
-        for (int i = 0; i < in_flight; ++i) {
-          if (--stage < 0) {
-            stage = C::kStages - 1;
-            phase ^= 1;
-          }
-          BarrierWait(SharedAddress(full_bar + stage), phase, &ignored);
+        __syncwarp();
+        ++issued;
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
     }
+    // After a failure the copies in flight still have to land.
+    if (!ok) {
+      volatile int ignored = 0;
+      const int in_flight =
+          static_cast<int>(issued < C::kStages ? issued : C::kStages);
+      for (int i = 0; i < in_flight; ++i) {
+        if (--stage < 0) {
+          stage = C::kStages - 1;
+          phase ^= 1;
+        }
+        BarrierWait(SharedAddress(full_bar + stage), phase, &ignored);
+      }
+    }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0, acc = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true;
-      for (int64_t item = first_item; ok && item < items; item += item_step) {
-        const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
-        ok = BarrierWait(SharedAddress(acc_empty_bar + acc), acc_phase ^ 1,
-                         &failed);
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int64_t item = first_item; ok && item < items; item += item_step) {
+      ok = BarrierWait(SharedAddress(acc_empty_bar + acc), acc_phase ^ 1,
+                       &failed);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      const uint32_t d = tmem + acc * C::kAccColumns;
+      for (int s = k_begin; s < k_end; ++s) {
+        ok = BarrierWait(SharedAddress(full_bar + stage), phase, &failed);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         FenceAfterSync();
-        const uint32_t d = tmem + acc * C::kAccColumns;
-        for (int s = k_begin; s < k_end; ++s) {
-          ok = BarrierWait(SharedAddress(full_bar + stage), phase, &failed);
-          if (!ok) break;
-          FenceAfterSync();
+        if (Elect()) {
           const uint32_t at = stage_base + stage * C::kStageBytes;
-          const uint32_t scales = at + kABytes + C::kBBytes;
           // The stage's own columns: they are free once its last MMAs are
           // done, which the stage's empty barrier has shown.
           const uint32_t a_col =
               tmem + C::kAccs * C::kAccColumns + stage * C::kScaleColumns;
           const uint32_t b_col = a_col + 8;
+          const uint64_t a_desc = SwizzledDesc(at);
+          const uint64_t b_desc = SwizzledDesc(at + kABytes);
+          const uint64_t scales = ScaleDesc(at + kABytes + C::kBBytes);
           const int left = p.k - s * kStageK;
-          const int steps = left >= kStageK ? 4 : (left + 63) / 64;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            if (h * 2 >= steps) break;
-            CopyScales(a_col + h * 4, ScaleDesc(scales + h * kMxTileBytes));
+            if (h * 128 >= left) break;
+            // Descriptors count 16 bytes.
+            CopyScales(a_col + h * 4, scales + h * (kMxTileBytes / 16));
 #pragma unroll
             for (int q = 0; q < C::kBTiles; ++q) {
               CopyScales(b_col + (h * C::kBTiles + q) * 4,
-                         ScaleDesc(scales + (1 + q) * kScaleBytes +
-                                   h * kMxTileBytes));
+                         scales + ((1 + q) * kScaleBytes + h * kMxTileBytes) /
+                                      16);
             }
           }
-          for (int j = 0; j < steps; ++j) {
-            Mma(d, SwizzledDesc(at + j * 32),
-                SwizzledDesc(at + kABytes + j * 32),
-                InstructionDesc<kN>(j & 1), a_col + (j >> 1) * 4,
-                b_col + (j >> 1) * 4 * C::kBTiles,
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j * 64 >= left) break;
+            Mma(d, a_desc + j * 2, b_desc + j * 2, InstructionDesc<kN>(j & 1),
+                a_col + (j >> 1) * 4, b_col + (j >> 1) * 4 * C::kBTiles,
                 s > k_begin || j > 0);
           }
           Commit(SharedAddress(empty_bar + stage));
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
-        if (!ok) break;
-        Commit(SharedAddress(acc_full_bar + acc));
-        if (++acc == C::kAccs) {
-          acc = 0;
-          acc_phase ^= 1;
+        __syncwarp();
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1;
         }
+      }
+      if (!ok) break;
+      if (Elect()) Commit(SharedAddress(acc_full_bar + acc));
+      __syncwarp();
+      if (++acc == C::kAccs) {
+        acc = 0;
+        acc_phase ^= 1;
       }
     }
   } else {
     // Tensor memory lanes [32 q, 32 q + 32) belong to warps with warp % 4 = q.
+    // A warp takes its columns into registers and gives the accumulator back
+    // before it stores them, so that the next tile's MMAs wait for the reads
+    // alone.
     const int quarter = warp & 3;
+    const int first_column = (warp - 2) / 4 * C::kPart;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int64_t item = first_item; item < items; item += item_step) {
       const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
-      const bool ok = BarrierWait(SharedAddress(acc_full_bar + acc), acc_phase,
-                                  &failed);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      FenceAfterSync();
       const int feature = t.m * kM + quarter * 32 + lane;
       const bool mine = feature < p.out;
-      const uint32_t d = tmem + acc * C::kAccColumns +
-                         (static_cast<uint32_t>(quarter * 32) << 16);
       const float bias =
           p.bias != nullptr && mine
               ? __ldg(p.bias + static_cast<int64_t>(t.group) * p.out + feature)
               : 0.0f;
-      if (p.split == 1) {
-        for (int c = 0; c < kN && c < t.rows; c += 16) {
-          float v[16];
-          LoadColumns<16>(d + c, v);
+      const bool ok = BarrierWait(SharedAddress(acc_full_bar + acc), acc_phase,
+                                  &failed);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      FenceAfterSync();
+      const uint32_t d = tmem + acc * C::kAccColumns + first_column +
+                         (static_cast<uint32_t>(quarter * 32) << 16);
+      const bool some = first_column < kN && first_column < t.rows;
+      uint32_t r[C::kPart];
+      if (some) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (mine && c + i < t.rows) {
-              StoreY(p, t.row + c + i, feature,
-                     Activate(v[i] + bias, p.activation));
-            }
-          }
-        }
-      } else {
-        // This block's part, [column][feature], over the stages (all read).
-        float* part = reinterpret_cast<float*>(stages);
-        for (int c = 0; c < kN && c < t.rows; c += 16) {
-          float v[16];
-          LoadColumns<16>(d + c, v);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            part[(c + i) * kM + quarter * 32 + lane] =
-                k_end > k_begin ? v[i] : 0.0f;
-          }
-        }
+        for (int c = 0; c < C::kPart; c += 16) LoadColumns(d + c, r + c);
+        WaitLoads();
       }
       FenceBeforeSync();
       __syncwarp();
@@ -560,16 +606,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         acc = 0;
         acc_phase ^= 1;
       }
+      if (!some) continue;
+      if (p.split == 1) {
+        T* y = static_cast<T*>(p.y) +
+               (t.row + first_column) * p.y_stride + feature;
+        const int rows = t.rows - first_column;
+#pragma unroll
+        for (int c = 0; c < C::kPart; c += 16) {
+          if (c >= rows) break;
+          StoreRows(y + c * p.y_stride, p.y_stride, r + c, bias, p.activation,
+                    rows - c, mine, p.paired, lane);
+        }
+      } else {
+        // This block's part, [column][feature], over the stages (all read).
+        float* part = reinterpret_cast<float*>(stages) + first_column * kM +
+                      quarter * 32 + lane;
+#pragma unroll
+        for (int c = 0; c < C::kPart; ++c) {
+          part[c * kM] = k_end > k_begin ? __uint_as_float(r[c]) : 0.0f;
+        }
+      }
     }
     // Rows behind the last group's.
     if (p.offsets != nullptr) {
       const int64_t kept = row_begin[p.groups];
       const int64_t total = (p.rows - kept) * p.out;
       const int thread = threadIdx.x - 64;
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * 128 + thread;
-           i < total; i += static_cast<int64_t>(gridDim.x) * 128) {
+      constexpr int kStep = 32 * kEpilogueWarps;
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStep + thread;
+           i < total; i += static_cast<int64_t>(gridDim.x) * kStep) {
         const int64_t r = i / p.out;
-        StoreY(p, kept + r, static_cast<int>(i - r * p.out), 0.0f);
+        Store(static_cast<T*>(p.y) + (kept + r) * p.y_stride + (i - r * p.out),
+              0.0f);
       }
     }
   }
@@ -585,12 +653,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           p.bias != nullptr && feature < p.out
               ? __ldg(p.bias + static_cast<int64_t>(t.group) * p.out + feature)
               : 0.0f;
-      for (int c = rank; c < t.rows; c += p.split) {
+      for (int c = rank * 2 + (warp - 2) / 4; c < t.rows; c += 2 * p.split) {
         const uint32_t at = stage_base + (c * kM + lane_feature) * 4;
         float sum = 0.0f;
         for (int b = 0; b < p.split; ++b) sum += LoadPeer(at, b);
         if (feature < p.out) {
-          StoreY(p, t.row + c, feature, Activate(sum + bias, p.activation));
+          Store(static_cast<T*>(p.y) + (t.row + c) * p.y_stride + feature,
+                Activate(sum + bias, p.activation));
         }
       }
     }
@@ -661,20 +730,20 @@ int EncodeCodes(CUtensorMap* map, const void* codes, int64_t row_bytes,
   return XSE_OK;
 }
 
-template <int kN>
-int LaunchGemm(GemmParams& p, int64_t codes_rows, const void* a_codes,
-               const void* b_codes, int64_t most_items, cudaStream_t s) {
+template <int kN, typename T>
+int LaunchGemmAs(GemmParams& p, const void* a_codes, const void* b_codes,
+                 int64_t most_items, cudaStream_t s) {
   using C = Config<kN>;
   const int64_t row_bytes = MxRowBytes(p.k);
   int rc = EncodeCodes(&p.a, a_codes, row_bytes, p.out, p.groups, 3, kM);
   if (rc == XSE_OK) {
-    rc = EncodeCodes(&p.b, b_codes, row_bytes, codes_rows, 1, 2, kN);
+    rc = EncodeCodes(&p.b, b_codes, row_bytes, p.rows, 1, 2, kN);
   }
   if (rc != XSE_OK) return rc;
   const size_t smem = 1024 + C::kStages * C::kStageBytes +
                       (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
   cudaError_t e = cudaFuncSetAttribute(
-      MxGemmKernel<kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      MxGemmKernel<kN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
       static_cast<int>(smem));
   if (e == cudaSuccess) {
     int64_t blocks = most_items * p.split;
@@ -690,7 +759,7 @@ int LaunchGemm(GemmParams& p, int64_t codes_rows, const void* a_codes,
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, MxGemmKernel<kN>, p);
+    e = cudaLaunchKernelEx(&cfg, MxGemmKernel<kN, T>, p);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -698,6 +767,15 @@ int LaunchGemm(GemmParams& p, int64_t codes_rows, const void* a_codes,
                     cudaGetErrorString(e));
   }
   return XSE_OK;
+}
+
+template <int kN>
+int LaunchGemm(GemmParams& p, int32_t y_dtype, const void* a_codes,
+               const void* b_codes, int64_t most_items, cudaStream_t s) {
+  return y_dtype == XSE_DT_BF16
+             ? LaunchGemmAs<kN, __nv_bfloat16>(p, a_codes, b_codes, most_items,
+                                               s)
+             : LaunchGemmAs<kN, float>(p, a_codes, b_codes, most_items, s);
 }
 
 // The product of rows in b (codes, scales) with w; plan NULL: one group.
@@ -721,7 +799,8 @@ int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
   p.k_stages = (w.cols + kStageK - 1) / kStageK;
   p.m_tiles = static_cast<int32_t>(MxRowTiles(w.rows));
   p.activation = activation;
-  p.y_bf16 = y_dtype == XSE_DT_BF16;
+  p.paired = y_dtype == XSE_DT_BF16 && (reinterpret_cast<uintptr_t>(y) & 3) == 0 &&
+             y_stride % 2 == 0 && w.rows % 2 == 0;
   p.split = 1;
   // Rows a group has on average decide the tile's rows.
   const int n = MxTileRowsFor(rows, p.groups);
@@ -738,13 +817,15 @@ int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
   }
   switch (n) {
     case 16:
-      return LaunchGemm<16>(p, rows, w.codes, b_codes, items, s);
+      return LaunchGemm<16>(p, y_dtype, w.codes, b_codes, items, s);
     case 32:
-      return LaunchGemm<32>(p, rows, w.codes, b_codes, items, s);
+      return LaunchGemm<32>(p, y_dtype, w.codes, b_codes, items, s);
     case 64:
-      return LaunchGemm<64>(p, rows, w.codes, b_codes, items, s);
+      return LaunchGemm<64>(p, y_dtype, w.codes, b_codes, items, s);
+    case 128:
+      return LaunchGemm<128>(p, y_dtype, w.codes, b_codes, items, s);
     default:
-      return LaunchGemm<128>(p, rows, w.codes, b_codes, items, s);
+      return LaunchGemm<256>(p, y_dtype, w.codes, b_codes, items, s);
   }
 }
 

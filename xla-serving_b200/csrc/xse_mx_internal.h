@@ -43,7 +43,8 @@ int CheckExpertPlan(const xse_expert_plan* plan);
 // many rows each, so that every tile's scales begin a column of tensor memory.
 inline int MxTileRowsFor(int64_t rows, int32_t groups) {
   const int64_t mean = (rows + groups - 1) / groups;
-  return mean <= 16 ? 16 : mean <= 32 ? 32 : mean <= 64 ? 64 : 128;
+  if (mean <= 64) return mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
+  return groups == 1 && mean > 128 ? 256 : 128;
 }
 
 // Scale tiles of n rows that hold every expert's rows on tile boundaries:
@@ -51,7 +52,7 @@ inline int MxTileRowsFor(int64_t rows, int32_t groups) {
 // tile offsets[e] / n + e + ceil(c / n) <= (offsets[e] + c) / n + e + 1, the
 // next one's start, so no scan of the counts is needed.
 inline int64_t ExpertScaleTiles(int64_t pairs, int32_t num_experts, int n) {
-  return pairs / n + num_experts;
+  return (pairs / n + num_experts) * (n > kMxTileRows ? 2 : 1);
 }
 
 // Quantises the rows of x for a product: plan NULL as xse_mxfp4_quantize of
