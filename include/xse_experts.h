@@ -42,9 +42,14 @@ typedef struct xse_expert_plan {
 
 /* Fills the plan's three arrays from ids [tokens, topk] (ids_type
  * XSE_INDEX_I32 or XSE_INDEX_I64, contiguous). tokens * topk < 2^31 and
- * 1 <= num_experts <= XSE_MAX_EXPERTS. */
+ * 1 <= num_experts <= XSE_MAX_EXPERTS. `workspace` holds
+ * xse_expert_sort_workspace(tokens * topk, num_experts) bytes (none for small
+ * batches: it may then be NULL), 4-byte aligned, used until the call's work on
+ * `stream` is done. */
+int64_t xse_expert_sort_workspace(int64_t pairs, int32_t num_experts);
 int xse_expert_sort(const void* ids, int32_t ids_type,
-                    const xse_expert_plan* plan, void* stream);
+                    const xse_expert_plan* plan, void* workspace,
+                    int64_t workspace_bytes, void* stream);
 
 /* out[r] = x[order[r] / topk] for every sorted row r, zeros behind the last:
  * x [tokens, cols], out [tokens * topk, cols]. Its gradient is

@@ -138,7 +138,8 @@ def test_layer_refusals(capi):
 
 def test_expert_refusals(capi):
   lib = capi.lib
-  sort = lambda p, kind=0, ids=4096: lib.xse_expert_sort(ids, kind, p, None)  # noqa: E731
+  sort = lambda p, kind=0, ids=4096, w=None, n=0: lib.xse_expert_sort(  # noqa: E731
+      ids, kind, p, w, n, None)
   refused(capi, sort(None), "plan")
   refused(capi, sort(plan(capi, tokens=-1)), "tokens")
   refused(capi, sort(plan(capi, topk=0)), "topk")
@@ -149,6 +150,12 @@ def test_expert_refusals(capi):
   refused(capi, sort(plan(capi, slots=None)), "non-null")
   refused(capi, sort(plan(capi), kind=2), "int32 or int64")
   refused(capi, sort(plan(capi), ids=None), "non-null")
+  need = lib.xse_expert_sort_workspace(100000, 3)
+  assert need > 0 and lib.xse_expert_sort_workspace(8, 3) == 0
+  large = plan(capi, tokens=50000)
+  refused(capi, sort(large), "workspace")
+  refused(capi, sort(large, w=4096, n=need - 1), "workspace")
+  refused(capi, sort(large, w=4098, n=need), "aligned")
 
   def gather(p=None, dtype=0, cols=64, x=4096, xs=64, out=4096, os=64):
     return lib.xse_expert_gather(x, dtype, cols, xs, p or plan(capi), out, os,

@@ -342,7 +342,8 @@ class ExpertPlanStruct(ctypes.Structure):
 
 _PLANP = ctypes.POINTER(ExpertPlanStruct)
 SIGNATURES.update({
-    "xse_expert_sort": (_I, [_P, _I32, _PLANP, _P]),
+    "xse_expert_sort_workspace": (_I64, [_I64, _I32]),
+    "xse_expert_sort": (_I, [_P, _I32, _PLANP, _P, _I64, _P]),
     "xse_expert_gather": (_I, [_P, _I32, _I32, _I64, _PLANP, _P, _I64, _P]),
     "xse_expert_combine": (_I, [_P, _I32, _I32, _I64, _PLANP, _P, _P, _I64,
                                 _P]),

@@ -1,17 +1,14 @@
 // Rows sorted by expert and back (include/xse_experts.h).
 //
-// Sorting is one launch: a cluster of up to eight blocks counts each warp's
-// pairs per expert in shared memory, the blocks read one another's totals over
-// distributed shared memory, and every warp then places its pairs in order.
+// Sorting counts each warp's pairs per expert in shared memory, turns the
+// counts into first rows, and lets every warp place its pairs in order; no
+// order depends on an atomic's. A block per SM, so that the scattered stores of
+// `order` spread over all of them (131072 pairs: 39 us in a cluster of eight).
 // The row movers work token by token, so that a token's row (or its gradient)
 // is read once for all its choices; their traffic is the rows themselves, each
 // read and written once, and they are bound by HBM bandwidth.
 
-#include <cooperative_groups.h>
-
 #include "xse_mx_internal.h"
-
-namespace cg = cooperative_groups;
 
 namespace xse {
 
@@ -41,148 +38,237 @@ namespace {
 
 constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortCluster = 8;
+constexpr int kSortLoads = 8;  // ids of a thread in flight
 
+// The expert of pair p, `num_experts` for a dropped one.
 template <typename Id>
-__device__ __forceinline__ int ExpertId(const Id* ids, int64_t p,
-                                        int num_experts) {
-  const Id id = ids[p];
-  return id >= 0 && id < num_experts ? static_cast<int>(id) : -1;
+__device__ __forceinline__ int ExpertId(Id id, int num_experts) {
+  return id >= 0 && id < num_experts ? static_cast<int>(id) : num_experts;
 }
 
-// Warp w of block b takes the pairs [(b * 32 + w) * per_warp, + per_warp).
-// Shared: counts[32][experts], then totals[experts] (this block's), then
-// starts[experts] (this block's first row of each expert).
+// A warp's pairs [first, last), 32 a step, the ids of kSortLoads steps in
+// registers: up to 256 pairs are loaded once for both passes over them.
+template <typename Id>
+struct WarpPairs {
+  const Id* ids;
+  int64_t first, last;
+  int num_experts, lane;
+  int expert[kSortLoads];
+
+  __device__ void Load(int64_t base) {
+#pragma unroll
+    for (int i = 0; i < kSortLoads; ++i) {
+      const int64_t p = base + 32 * i + lane;
+      expert[i] =
+          p < last ? ExpertId(__ldg(ids + p), num_experts) : num_experts;
+    }
+  }
+  // Calls step(p, expert) for every pair; all lanes take every step, those
+  // past `last` with a dropped pair.
+  template <typename Step>
+  __device__ void ForEach(bool loaded, Step step) {
+    for (int64_t base = first; base < last; base += 32 * kSortLoads) {
+      if (!loaded) Load(base);
+#pragma unroll
+      for (int i = 0; i < kSortLoads; ++i) {
+        if (base + 32 * i >= last) break;
+        step(base + 32 * i + lane, expert[i]);
+      }
+    }
+  }
+  __device__ bool Once() const { return last - first <= 32 * kSortLoads; }
+};
+
+// Warp w of block b takes the pairs [(b * warps + w) * per_warp, + per_warp).
+// With several blocks, a first launch counts each block's pairs per expert.
+template <typename Id>
+__global__ void __launch_bounds__(kSortThreads)
+    SortCountKernel(const Id* __restrict__ ids, int pairs, int num_experts,
+                    int64_t per_warp, int32_t* __restrict__ counts) {
+  extern __shared__ int totals[];
+  // The next launch may begin; it waits for the counts where it reads them.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = threadIdx.x; e < num_experts; e += kSortThreads) totals[e] = 0;
+  __syncthreads();
+  const int64_t first =
+      (static_cast<int64_t>(blockIdx.x) * kSortWarps + threadIdx.x / 32) *
+      per_warp;
+  WarpPairs<Id> mine{ids, first,
+                     min(first + per_warp, static_cast<int64_t>(pairs)),
+                     num_experts, static_cast<int>(threadIdx.x & 31)};
+  mine.ForEach(false, [&](int64_t, int e) {
+    if (e < num_experts) atomicAdd(totals + e, 1);
+  });
+  __syncthreads();
+  for (int e = threadIdx.x; e < num_experts; e += kSortThreads) {
+    counts[static_cast<int64_t>(blockIdx.x) * num_experts + e] = totals[e];
+  }
+}
+
+// Each warp counts its pairs per expert, the counts become its first rows, and
+// it then places its pairs in order, lanes of one expert by rank. `counts`:
+// every block's from the launch before, NULL for one block.
+// Shared: counts[warps][experts], all[experts], before[experts] (all pairs of
+// an expert, and those of the blocks before this one).
 template <typename Id>
 __global__ void __launch_bounds__(kSortThreads)
     SortKernel(const Id* __restrict__ ids, int pairs, int num_experts,
-               int64_t per_warp, int32_t* __restrict__ offsets,
-               int32_t* __restrict__ order, int32_t* __restrict__ slots) {
+               int64_t per_warp, const int32_t* counts,
+               int32_t* __restrict__ offsets, int32_t* __restrict__ order,
+               int32_t* __restrict__ slots) {
   extern __shared__ int shared[];
   __shared__ int warp_sums[kSortWarps];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int blocks = gridDim.x;  // one cluster
-  const int block = blockIdx.x;
+  const int block = blockIdx.x, blocks = gridDim.x;
+  const int threads = blockDim.x, warps = threads / 32;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31;
   int* mine = shared + warp * num_experts;
-  int* totals = shared + kSortWarps * num_experts;
-  int* starts = totals + num_experts;
-  for (int i = threadIdx.x; i < kSortWarps * num_experts; i += kSortThreads) {
+  int* all = shared + warps * num_experts;
+  int* before = all + num_experts;
+  const int64_t first =
+      (static_cast<int64_t>(block) * warps + warp) * per_warp;
+  WarpPairs<Id> part{ids, first,
+                     min(first + per_warp, static_cast<int64_t>(pairs)),
+                     num_experts, lane};
+  const bool once = part.Once();
+  if (once) part.Load(first);
+  for (int i = threadIdx.x; i < (warps + 2) * num_experts; i += threads) {
     shared[i] = 0;
   }
   __syncthreads();
-  const int64_t first =
-      (static_cast<int64_t>(block) * kSortWarps + warp) * per_warp;
-  const int64_t last = min(first + per_warp, static_cast<int64_t>(pairs));
-  for (int64_t p = first + lane; p - lane < last; p += 32) {
-    const int e = p < last ? ExpertId(ids, p, num_experts) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+  part.ForEach(once, [&](int64_t, int e) {
+    if (e < num_experts) atomicAdd(mine + e, 1);
+  });
+  if (counts != nullptr) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // Warps share the experts (32 at a time) and, where there are more warps
+    // than that, the blocks.
+    const int chunks = (num_experts + 31) / 32;
+    const int groups = chunks < warps ? warps / chunks : 1;
+    for (int chunk = warp / groups; chunk < chunks; chunk += warps / groups) {
+      const int e = chunk * 32 + lane;
+      if (e >= num_experts) continue;
+      int sum = 0, earlier = 0;
+#pragma unroll 8
+      for (int b = warp % groups; b < blocks; b += groups) {
+        const int c = counts[static_cast<int64_t>(b) * num_experts + e];
+        sum += c;
+        if (b < block) earlier += c;
+      }
+      if (sum != 0) atomicAdd(all + e, sum);
+      if (earlier != 0) atomicAdd(before + e, earlier);
+    }
   }
   __syncthreads();
-  // Counts before each warp, within the block.
-  for (int e = threadIdx.x; e < num_experts; e += kSortThreads) {
-    int sum = 0;
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int c = shared[w * num_experts + e];
-      shared[w * num_experts + e] = sum;
-      sum += c;
+  // Experts in turn: counts before each warp within the block, a scan over
+  // the experts, and each warp's first row.
+  int carry = 0;
+  for (int base = 0; base < num_experts; base += threads) {
+    const int e = base + threadIdx.x;
+    int total = 0;
+    if (e < num_experts) {
+      int sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < warps; ++w) {
+        const int c = shared[w * num_experts + e];
+        shared[w * num_experts + e] = sum;
+        sum += c;
+      }
+      total = counts != nullptr ? all[e] : sum;
     }
-    totals[e] = sum;
-  }
-  if (blocks > 1) {
-    cluster.sync();
-  } else {
+    int scan = total;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += up;
+    }
+    if (lane == 31) warp_sums[warp] = scan;
+    __syncthreads();
+    int sums = lane < warps ? warp_sums[lane] : 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sums, o);
+      if (lane >= o) sums += up;
+    }
+    const int earlier = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+    const int begin = carry + scan - total + (warp > 0 ? earlier : 0);
+    carry += __shfl_sync(0xffffffffu, sums, 31);
+    if (e < num_experts) {
+      if (block == 0) {
+        offsets[e] = begin;
+        if (e == num_experts - 1) offsets[num_experts] = begin + total;
+      }
+      before[e] += begin;
+    }
     __syncthreads();
   }
-  // Thread e: all rows of expert e, and those of the blocks before this one;
-  // then a scan over the experts (at most one per thread).
-  int all = 0, before = 0;
-  const int e = threadIdx.x;
-  if (e < num_experts) {
-    for (int b = 0; b < blocks; ++b) {
-      const int c = blocks > 1 ? *cluster.map_shared_rank(totals + e, b)
-                               : totals[e];
-      if (b < block) before += c;
-      all += c;
+  const int bits = 32 - __clz(num_experts);
+  part.ForEach(once, [&](int64_t p, int e) {
+    // Lanes of the same expert, one vote per bit of its number.
+    unsigned same = 0xffffffffu;
+    for (int b = 0; b < bits; ++b) {
+      const bool set = e >> b & 1;
+      const unsigned votes = __ballot_sync(0xffffffffu, set);
+      same &= set ? votes : ~votes;
     }
-  }
-  int scan = all;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += up;
-  }
-  if (lane == 31) warp_sums[warp] = scan;
-  __syncthreads();
-  int base = 0;
-  for (int w = 0; w < warp; ++w) base += warp_sums[w];
-  int kept = 0;
-  for (int w = 0; w < kSortWarps; ++w) kept += warp_sums[w];
-  if (e < num_experts) {
-    const int begin = base + scan - all;
-    starts[e] = begin + before;
-    if (block == 0) {
-      offsets[e] = begin;
-      if (e == num_experts - 1) offsets[num_experts] = begin + all;
-    }
-  }
-  __syncthreads();
-  for (int64_t p = first + lane; p - lane < last; p += 32) {
-    const int id = p < last ? ExpertId(ids, p, num_experts) : -1;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
     const int rank = __popc(same & ((1u << lane) - 1u));
     int row = -1;
-    if (id >= 0) {
-      row = starts[id] + mine[id] + rank;
+    if (e < num_experts) {
+      row = before[e] + mine[e] + rank;
       order[row] = static_cast<int32_t>(p);
     }
-    if (p < last) slots[p] = row;
+    if (p < part.last) slots[p] = row;
     __syncwarp();
-    if (id >= 0 && rank == 0) mine[id] += __popc(same);
+    if (e < num_experts && rank == 0) mine[e] += __popc(same);
     __syncwarp();
-  }
-  for (int64_t r = static_cast<int64_t>(kept) + block * kSortThreads +
-                   threadIdx.x;
-       r < pairs; r += blocks * kSortThreads) {
+  });
+  for (int64_t r = static_cast<int64_t>(carry) + block * threads + threadIdx.x;
+       r < pairs; r += blocks * threads) {
     order[r] = -1;
   }
-  // A block's totals stay until the others have read them.
-  if (blocks > 1) cluster.sync();
+}
+
+// Pairs that one block sorts in one launch; more take a block per SM and two.
+// 4096 pairs over 128 experts: 8.3 us in one block, 6.7 us in two launches.
+constexpr int kSortOneBlock = 2048;
+
+int SortBlocks(int64_t pairs) {
+  if (pairs <= kSortOneBlock) return 1;
+  const int64_t blocks = (pairs + kSortThreads - 1) / kSortThreads;
+  return static_cast<int>(blocks > kNumSms ? kNumSms : blocks);
 }
 
 template <typename Id>
-int LaunchSort(const void* ids, const xse_expert_plan& plan, cudaStream_t s) {
+cudaError_t LaunchSort(const Id* ids, const xse_expert_plan& plan,
+                       int32_t* counts, cudaStream_t s) {
   const int pairs = static_cast<int>(plan.tokens * plan.topk);
-  const int blocks = pairs > 4096 ? kSortCluster : 1;
-  int64_t per_warp = (pairs + blocks * kSortWarps - 1) / (blocks * kSortWarps);
+  const int blocks = SortBlocks(pairs);
+  const int threads = pairs <= 512 ? 256 : kSortThreads, warps = threads / 32;
+  int64_t per_warp = (pairs + blocks * warps - 1) / (blocks * warps);
   per_warp = (per_warp + 31) / 32 * 32;
-  const size_t smem = sizeof(int) * (kSortWarps + 2) *
-                      static_cast<size_t>(plan.num_experts);
+  const size_t row = sizeof(int) * static_cast<size_t>(plan.num_experts);
   cudaError_t e = cudaFuncSetAttribute(
       SortKernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      static_cast<int>(smem));
-  if (e == cudaSuccess) {
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(blocks);
-    cfg.blockDim = dim3(kSortThreads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = blocks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, SortKernel<Id>, static_cast<const Id*>(ids),
-                           pairs, static_cast<int>(plan.num_experts), per_warp,
-                           plan.offsets, plan.order, plan.slots);
+      static_cast<int>(sizeof(int) * (kSortWarps + 2) * XSE_MAX_EXPERTS));
+  if (e != cudaSuccess) return e;
+  if (blocks > 1) {
+    SortCountKernel<Id><<<blocks, kSortThreads, row, s>>>(
+        ids, pairs, plan.num_experts, per_warp, counts);
   }
-  if (e != cudaSuccess) cudaGetLastError();
-  return e == cudaSuccess ? XSE_OK
-                          : FailWith(XSE_INTERNAL, "expert sort launch: %s",
-                                     cudaGetErrorString(e));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = (warps + 2) * row;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = blocks > 1 ? 1 : 0;
+  e = cudaLaunchKernelEx(
+      &cfg, SortKernel<Id>, ids, pairs, static_cast<int>(plan.num_experts),
+      per_warp, static_cast<const int32_t*>(blocks > 1 ? counts : nullptr),
+      plan.offsets, plan.order, plan.slots);
+  return e != cudaSuccess ? e : cudaGetLastError();
 }
 
 // --------------------------------------------------------------- row movers
@@ -822,8 +908,18 @@ constexpr char kNull[] = "Expert row buffers must be non-null.";
 
 extern "C" {
 
+int64_t xse_expert_sort_workspace(int64_t pairs, int32_t num_experts) {
+  if (pairs < 0 || pairs > INT32_MAX || num_experts < 1 ||
+      num_experts > XSE_MAX_EXPERTS) {
+    return 0;
+  }
+  const int blocks = xse::SortBlocks(pairs);
+  return blocks == 1 ? 0 : int64_t{4} * blocks * num_experts;
+}
+
 int xse_expert_sort(const void* ids, int32_t ids_type,
-                    const xse_expert_plan* plan, void* stream) {
+                    const xse_expert_plan* plan, void* workspace,
+                    int64_t workspace_bytes, void* stream) {
   using namespace xse;
   SetLastLaunchCount(0);
   if (int rc = CheckExpertPlan(plan); rc != XSE_OK) return rc;
@@ -834,11 +930,28 @@ int xse_expert_sort(const void* ids, int32_t ids_type,
   if (plan->tokens > 0 && ids == nullptr) {
     return FailWith(XSE_INVALID_ARGUMENT, "Expert ids must be non-null.");
   }
+  const int64_t need = xse_expert_sort_workspace(plan->tokens * plan->topk,
+                                                 plan->num_experts);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need ||
+                   (reinterpret_cast<uintptr_t>(workspace) & 3) != 0)) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "Expert sort needs a 4-byte aligned workspace of %lld "
+                    "bytes, got %lld.", static_cast<long long>(need),
+                    static_cast<long long>(workspace_bytes));
+  }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int rc = ids_type == XSE_INDEX_I64 ? LaunchSort<long long>(ids, *plan, s)
-                                           : LaunchSort<int>(ids, *plan, s);
-  if (rc == XSE_OK) SetLastLaunchCount(1);
-  return rc;
+  int32_t* counts = static_cast<int32_t*>(workspace);
+  const cudaError_t e =
+      ids_type == XSE_INDEX_I64
+          ? LaunchSort(static_cast<const long long*>(ids), *plan, counts, s)
+          : LaunchSort(static_cast<const int*>(ids), *plan, counts, s);
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return FailWith(XSE_INTERNAL, "expert sort launch: %s",
+                    cudaGetErrorString(e));
+  }
+  SetLastLaunchCount(need > 0 ? 2 : 1);
+  return XSE_OK;
 }
 
 int xse_expert_gather(const void* x, int32_t dtype, int32_t cols,

@@ -5,15 +5,10 @@
 // arithmetic is exact (a power of two times a float) except the one rounding
 // to E2M1, so results do not depend on the kernel that ran.
 //
-// Three kernels read rows that differ in what their loads can be:
-//   QuantizeVecKernel   16-byte aligned rows: a lane takes 8 elements, four
-//                       lanes share a block
-//   QuantizeWarpKernel  rows at any alignment: a lane takes one element of
-//                       each of four blocks, so that loads stay coalesced, and
-//                       the codes are transposed to words with shuffles
-//   QuantizeStrideKernel  columns apart (a [in, out] kernel read as [out,
-//                       in]): a thread takes one block, neighbouring threads
-//                       neighbouring rows
+// Two kernels: QuantizeKernel for rows of neighbouring elements (a lane takes
+// 64 bytes of a row), QuantizeStrideKernel for elements apart (a [in, out]
+// kernel read as [out, in]: a thread takes one block, neighbouring threads
+// neighbouring rows).
 
 #include <cstdarg>
 #include <cstdio>
@@ -111,7 +106,8 @@ struct QuantParams {
   int32_t k_tiles;
   int64_t row_bytes;
   int64_t row_tiles;    // scale tiles of a group's rows (of all: with a plan)
-  int32_t tile_rows;    // rows of a scale tile
+  int32_t tile_rows;    // rows of a product's tile (2^tile_shift)
+  int32_t tile_shift;
   uint8_t* codes;
   uint8_t* scales;
   const int32_t* offsets;
@@ -130,22 +126,50 @@ __device__ __forceinline__ float ToFloat(__nv_bfloat16 v) {
   return __bfloat162float(v);
 }
 
-// Eight neighbouring elements (16-byte aligned).
-__device__ __forceinline__ void Load8(const float* p, float (&v)[8]) {
-  const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-  const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void Load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+// The 64 bytes of a row that a lane quantises: a whole block of bfloat16, half
+// a block of float32 (two lanes then agree on the scale).
+template <typename T>
+struct Part {
+  static constexpr int kElements = 64 / sizeof(T);
+  static constexpr int kLanes = kMxBlock / kElements;  // of a block
+  static constexpr int kWords = kElements / 8;         // of codes
+  uint4 v[4];
+
+  // The scale byte of the block and this lane's codes.
+  __device__ uint32_t Quantize(uint32_t (&codes)[kWords]) const {
+    const uint32_t* w = &v[0].x;
+    uint32_t most = 0;
+    if constexpr (sizeof(T) == 2) {
+      // Magnitudes are ordered as 16-bit integers, infinities and NaN last.
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    v[2 * i] = __uint_as_float(w[i] << 16);
-    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+      for (int i = 0; i < 16; ++i) {
+        most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+      }
+      most = max(most & 0xffff0000u, most << 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) most = max(most, w[i] & 0x7fffffffu);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    }
+    const uint32_t s = MxScaleByte(most);
+    const float inv = MxInverseScale(s);
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) {
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t u = w[4 * k + i / 2];
+          f[i] = __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16) * inv;
+        } else {
+          f[i] = __uint_as_float(w[8 * k + i]) * inv;
+        }
+      }
+      codes[k] = s == 255u ? 0u : MxCodes8(f);
+    }
+    return s;
   }
-}
+};
 
 template <typename T>
 __device__ __forceinline__ const T* RowOf(const QuantParams& p, int64_t row) {
@@ -172,10 +196,11 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
       if (e >= p.num_experts) continue;  // behind the last sorted row
       const int32_t begin = __ldg(p.offsets + e);
       if (begin < 0 || begin > slot) continue;
+      // tile_rows is a power of two; a tile of 256 rows has two scale tiles.
       const int local = slot - begin;
-      const int in_tile = local % p.tile_rows;
+      const int in_tile = local & (p.tile_rows - 1);
       const int64_t tile =
-          (begin / p.tile_rows + e + local / p.tile_rows) *
+          ((begin >> p.tile_shift) + e + (local >> p.tile_shift)) *
               (p.tile_rows > kMxTileRows ? 2 : 1) + in_tile / kMxTileRows;
       if (tile >= p.row_tiles) continue;
       put(static_cast<int64_t>(slot),
@@ -184,125 +209,81 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
   }
 }
 
-// A warp takes 512 columns of a row, a lane 8 of each half; four lanes share a
-// block and agree on its largest magnitude with two shuffles.
-template <typename T, int kMode>
+// A warp takes 32 parts of a row at a time. kAligned: a lane's 64 bytes are
+// loaded as they lie, four 16-byte loads that share cache lines with the
+// neighbouring lanes' (any split that keeps the loads contiguous over the warp
+// needs shuffles for the blocks' magnitudes and, worse, one scale per 8
+// elements: 31 us against KA us for 8192 x 4096 bf16). Otherwise the elements
+// are loaded one by one over the warp and turned through shared memory.
+template <typename T, int kMode, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
-    QuantizeVecKernel(const __grid_constant__ QuantParams p) {
+    QuantizeKernel(const __grid_constant__ QuantParams p) {
+  using P = Part<T>;
+  constexpr int kSpan = 32 * P::kElements;
+  __shared__ uint4 turn[kAligned ? 1 : kThreads / 32][kAligned ? 1 : 128];
   const int lane = threadIdx.x & 31;
   const int padded = p.k_tiles * 128, code_cols = (p.cols + 31) / 32 * 32;
   const WarpRow w = FirstRow(p.row_shift);
   for (int64_t row = w.row; row < p.total_rows; row += w.step) {
     const T* x = RowOf<T>(p, row);
-    for (int first = w.chunk * 512; first < padded; first += w.chunks * 512) {
-      float v[2][8];
+    for (int first = w.chunk * kSpan; first < padded;
+         first += w.chunks * kSpan) {
+      const int col = first + lane * P::kElements;
+      P part;
+      if constexpr (kAligned) {
+        const uint4* src = reinterpret_cast<const uint4*>(x + col);
+        if (col + P::kElements <= p.cols) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int col = first + h * 256 + lane * 8;
-        if (col + 8 <= p.cols) {
-          Load8(x + col, v[h]);
+          for (int i = 0; i < 4; ++i) part.v[i] = __ldg(src + i);
         } else {
+          T* e = reinterpret_cast<T*>(part.v);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            v[h][i] = col + i < p.cols ? ToFloat(x[col + i]) : 0.0f;
+          for (int i = 0; i < P::kElements; ++i) {
+            e[i] = col + i < p.cols ? x[col + i] : static_cast<T>(0.0f);
           }
         }
-      }
-      uint32_t word[2], scales[2];
+      } else {
+        // 16-byte piece c lies at c ^ (c / 8 % 4), so that neither the stores
+        // nor the lanes' loads meet in a bank.
+        T* mine = reinterpret_cast<T*>(turn[threadIdx.x / 32]);
+        constexpr int kPiece = 16 / sizeof(T);
+        T v[P::kElements];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          most = max(most, __float_as_uint(v[h][i]) & 0x7fffffffu);
+        for (int i = 0; i < P::kElements; ++i) {
+          const int c = first + 32 * i + lane;
+          v[i] = c < p.cols ? x[c] : static_cast<T>(0.0f);
         }
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const uint32_t s = MxScaleByte(most);
-        const float inv = MxInverseScale(s);
+        __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[h][i] *= inv;
-        word[h] = s == 255u ? 0u : MxCodes8(v[h]);
-        // The scale bytes of four blocks (16 lanes) as one word.
-        scales[h] = s | __shfl_down_sync(0xffffffffu, s, 4) << 8;
-        scales[h] |= __shfl_down_sync(0xffffffffu, scales[h], 8) << 16;
+        for (int i = 0; i < P::kElements; ++i) {
+          const int e = 32 * i + lane, piece = e / kPiece;
+          mine[(piece ^ (piece >> 3 & 3)) * kPiece + e % kPiece] = v[i];
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int piece = lane * 4 + i;
+          part.v[i] = turn[threadIdx.x / 32][piece ^ (piece >> 3 & 3)];
+        }
       }
+      uint32_t codes[P::kWords];
+      uint32_t scales = part.Quantize(codes);
+      // The scale bytes of four blocks as one word.
+      scales |= __shfl_down_sync(0xffffffffu, scales, P::kLanes) << 8;
+      scales |= __shfl_down_sync(0xffffffffu, scales, 2 * P::kLanes) << 16;
       ForPlaces<kMode>(p, row, lane, [&](int64_t code_row, int64_t scale_row) {
-        uint8_t* codes = p.codes + code_row * p.row_bytes;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int col = first + h * 256 + lane * 8;
-          if (col < code_cols) {
-            *reinterpret_cast<uint32_t*>(codes + col / 2) = word[h];
-          }
-          if ((lane & 15) == 0 && col < padded) {
-            *reinterpret_cast<uint32_t*>(
-                p.scales + MxScaleAt(scale_row, col / 32, p.k_tiles)) =
-                scales[h];
+        if (col < code_cols) {
+          uint8_t* dst = p.codes + code_row * p.row_bytes + col / 2;
+          if constexpr (P::kWords == 4) {
+            *reinterpret_cast<uint4*>(dst) =
+                make_uint4(codes[0], codes[1], codes[2], codes[3]);
+          } else {
+            *reinterpret_cast<uint2*>(dst) = make_uint2(codes[0], codes[1]);
           }
         }
-      });
-    }
-  }
-}
-
-// A warp takes 256 columns of a row as two halves of four blocks of 32 lanes.
-// Lane l ends with the word of block 2 (l & 1) + (l >> 1 & 1) of each half,
-// bytes 4 (l >> 3) on.
-template <typename T, int kMode>
-__global__ void __launch_bounds__(kThreads)
-    QuantizeWarpKernel(const __grid_constant__ QuantParams p) {
-  const unsigned all = 0xffffffffu;
-  const int lane = threadIdx.x & 31;
-  const bool odd = lane & 1, odd2 = lane & 2;
-  const int padded = p.k_tiles * 128, code_cols = (p.cols + 31) / 32 * 32;
-  const WarpRow w = FirstRow(p.row_shift);
-  for (int64_t row = w.row; row < p.total_rows; row += w.step) {
-    const T* x = RowOf<T>(p, row);
-    for (int first = w.chunk * 256; first < padded; first += w.chunks * 256) {
-      float v[8];
-#pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const int col = first + 32 * b + lane;
-        v[b] = col < p.cols ? ToFloat(x[col]) : 0.0f;
-      }
-      uint32_t word[2], scales[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float* u = v + 4 * h;
-        scales[h] = 0;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const uint32_t s = MxScaleByte(
-              __reduce_max_sync(all, __float_as_uint(u[b]) & 0x7fffffffu));
-          scales[h] |= s << (8 * b);
-          u[b] = s == 255u ? 0.0f : u[b] * MxInverseScale(s);
-        }
-        // Even lanes keep blocks 0 and 1, odd lanes 2 and 3, of a pair of
-        // elements; then each lane one block of two pairs; then of four.
-        const float r0 = __shfl_xor_sync(all, odd ? u[0] : u[2], 1);
-        const float r1 = __shfl_xor_sync(all, odd ? u[1] : u[3], 1);
-        const uint32_t b0 = odd ? MxCodes2(r0, u[2]) : MxCodes2(u[0], r0);
-        const uint32_t b1 = odd ? MxCodes2(r1, u[3]) : MxCodes2(u[1], r1);
-        const uint32_t got = __shfl_xor_sync(all, odd2 ? b0 : b1, 2);
-        word[h] = odd2 ? (got | b1 << 8) : (b0 | got << 8);
-        word[h] |= __shfl_down_sync(all, word[h], 4) << 16;
-      }
-      const int block = (odd ? 2 : 0) + (odd2 ? 1 : 0);
-      ForPlaces<kMode>(p, row, lane, [&](int64_t code_row, int64_t scale_row) {
-        uint8_t* codes = p.codes + code_row * p.row_bytes;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int half = first + 128 * h;
-          const int col = half + 32 * block + 8 * (lane >> 3);
-          if ((lane & 4) == 0 && col < code_cols) {
-            *reinterpret_cast<uint32_t*>(codes + col / 2) = word[h];
-          }
-          if (lane == 0 && half < padded) {
-            *reinterpret_cast<uint32_t*>(
-                p.scales + MxScaleAt(scale_row, half / 32, p.k_tiles)) =
-                scales[h];
-          }
+        if (lane % (4 * P::kLanes) == 0 && col < padded) {
+          *reinterpret_cast<uint32_t*>(
+              p.scales + MxScaleAt(scale_row, col / 32, p.k_tiles)) = scales;
         }
       });
     }
@@ -349,16 +330,44 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// A warp takes 256 columns of a row: its lanes load a word of eight codes
-// each, and every lane takes its element's word by a shuffle, so that the
-// stores are coalesced at any alignment.
+// The values of eight codes as pairs of bfloat16 (exact): two byte tables by
+// the low three bits of four codes at a time, then the signs.
+__device__ __forceinline__ void DecodeCodes(uint32_t word, uint32_t (&v)[4]) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t u = h ? word >> 16 : word;
+    const uint32_t pick = u & 0x7777u;
+    const uint32_t low = __byte_perm(0xc0800000u, 0xc0804000u, pick);
+    const uint32_t high = __byte_perm(0x3f3f3f00u, 0x40404040u, pick);
+    v[2 * h] = __byte_perm(low, high, 0x5140) | (u << 12 & 0x8000u) |
+               (u << 24 & 0x80000000u);
+    v[2 * h + 1] = __byte_perm(low, high, 0x7362) | (u << 4 & 0x8000u) |
+                   (u << 16 & 0x80000000u);
+  }
+}
+
 template <typename T>
+__device__ __forceinline__ T FromFloat(float v);
+template <>
+__device__ __forceinline__ float FromFloat(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 FromFloat(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// A warp takes 256 columns of a row, a lane eight of one block. kAligned: it
+// stores them whole; otherwise they are turned through shared memory, so that
+// the warp stores neighbouring elements.
+template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     DequantizeKernel(const uint8_t* __restrict__ codes,
                      const uint8_t* __restrict__ scales, int64_t rows,
                      int groups, int cols, int64_t row_bytes, int k_tiles,
                      int64_t row_tiles, int row_shift, T* __restrict__ out,
                      int64_t group_stride, int64_t row_stride) {
+  constexpr int kPiece = 16 / sizeof(T), kPieces = 8 / kPiece;
+  __shared__ uint4 turn[kAligned ? 1 : kThreads / 32]
+                       [kAligned ? 1 : 32 * kPieces];
   const int lane = threadIdx.x & 31;
   const int padded = k_tiles * 128;
   const WarpRow w = FirstRow(row_shift);
@@ -366,29 +375,59 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t g = groups == 1 ? 0 : row / rows;
     const int64_t r = row - g * rows;
     T* o = out + g * group_stride + r * row_stride;
+    const uint8_t* row_scales =
+        scales + MxScaleAt(g * row_tiles * kMxTileRows + r, 0, k_tiles);
     for (int first = w.chunk * 256; first < padded; first += w.chunks * 256) {
-      const int at = first / 2 + lane * 4;
-      const uint32_t word =
-          at < row_bytes
-              ? __ldg(reinterpret_cast<const uint32_t*>(codes +
-                                                        row * row_bytes + at))
-              : 0u;
-      uint32_t sc[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        sc[h] = first + 128 * h < padded
-                    ? __ldg(reinterpret_cast<const uint32_t*>(
-                          scales + MxScaleAt(g * row_tiles * kMxTileRows + r,
-                                             first / 32 + 4 * h, k_tiles)))
-                    : 0u;
+      const int col = first + lane * 8;
+      uint32_t word = 0, s = 0;
+      if (col < cols) {
+        word = __ldg(reinterpret_cast<const uint32_t*>(
+            codes + row * row_bytes + col / 2));
+        s = __ldg(row_scales + col / 128 * kMxTileBytes + col / 32 % 4);
       }
+      const float scale = MxScale(s);
+      uint32_t v[4];
+      DecodeCodes(word, v);
+      alignas(16) T e[8];
 #pragma unroll
-      for (int b = 0; b < 8; ++b) {
-        const uint32_t u = __shfl_sync(0xffffffffu, word, 4 * b + (lane >> 3));
-        const int col = first + 32 * b + lane;
-        const float v = MxCodeValue(u >> (4 * (lane & 7))) *
-                        MxScale(sc[b >> 2] >> (8 * (b & 3)) & 0xffu);
-        if (col < cols) o[col] = static_cast<T>(v);
+      for (int i = 0; i < 4; ++i) {
+        e[2 * i] = FromFloat<T>(__uint_as_float(v[i] << 16) * scale);
+        e[2 * i + 1] =
+            FromFloat<T>(__uint_as_float(v[i] & 0xffff0000u) * scale);
+      }
+      const uint4* pieces = reinterpret_cast<const uint4*>(e);
+      if constexpr (kAligned) {
+        if (col + 8 <= cols) {
+#pragma unroll
+          for (int i = 0; i < kPieces; ++i) {
+            reinterpret_cast<uint4*>(o + col)[i] = pieces[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            if (col + i < cols) o[col + i] = e[i];
+          }
+        }
+      } else {
+        // Piece c lies at c ^ (c / 8 % 2): two pieces of a lane, 32 bytes
+        // apart from the next lane's, then meet in no bank.
+        uint4* mine = turn[threadIdx.x / 32];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          const int c = lane * kPieces + i;
+          mine[kPieces == 2 ? c ^ (c >> 3 & 1) : c] = pieces[i];
+        }
+        __syncwarp();
+        const T* values = reinterpret_cast<const T*>(mine);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int at = 32 * i + lane, c = at / kPiece;
+          const T value =
+              values[(kPieces == 2 ? c ^ (c >> 3 & 1) : c) * kPiece +
+                     at % kPiece];
+          if (first + at < cols) o[first + at] = value;
+        }
       }
     }
   }
@@ -401,14 +440,32 @@ int BlocksFor(int64_t work, int per_block) {
 }
 
 template <typename T, int kMode>
-void LaunchQuantize(QuantParams p, bool vec, cudaStream_t s) {
-  p.row_shift = RowShift(vec ? (p.k_tiles + 3) / 4 : (p.k_tiles + 1) / 2);
+void LaunchQuantize(QuantParams p, bool aligned, cudaStream_t s) {
+  constexpr int kSpan = 32 * Part<T>::kElements;
+  p.row_shift = RowShift((p.k_tiles * 128 + kSpan - 1) / kSpan);
   const int blocks = BlocksForRows(p.total_rows, p.row_shift);
-  if (vec) {
-    QuantizeVecKernel<T, kMode><<<blocks, kThreads, 0, s>>>(p);
+  if (aligned) {
+    QuantizeKernel<T, kMode, true><<<blocks, kThreads, 0, s>>>(p);
   } else {
-    QuantizeWarpKernel<T, kMode><<<blocks, kThreads, 0, s>>>(p);
+    QuantizeKernel<T, kMode, false><<<blocks, kThreads, 0, s>>>(p);
   }
+}
+
+template <typename T>
+void LaunchDequantize(const xse_mx_matrix& q, void* out, int64_t group_stride,
+                      int64_t row_stride, cudaStream_t s) {
+  const int k_tiles = static_cast<int>(MxKTiles(q.cols));
+  const int row_shift = RowShift((k_tiles + 1) / 2);
+  const int64_t per = 16 / sizeof(T);
+  const bool aligned = Aligned16(out) && row_stride % per == 0 &&
+                       (q.groups == 1 || group_stride % per == 0);
+  const auto kernel =
+      aligned ? DequantizeKernel<T, true> : DequantizeKernel<T, false>;
+  kernel<<<BlocksForRows(q.rows * q.groups, row_shift), kThreads, 0, s>>>(
+      static_cast<const uint8_t*>(q.codes),
+      static_cast<const uint8_t*>(q.scales), q.rows, q.groups, q.cols,
+      MxRowBytes(q.cols), k_tiles, MxRowTiles(q.rows), row_shift,
+      static_cast<T*>(out), group_stride, row_stride);
 }
 
 template <typename T>
@@ -454,6 +511,7 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
   if (plan == nullptr) return RunQuantize(p, dtype, kPlain, stream);
   p.pairs = plan->tokens * plan->topk;
   p.tile_rows = MxTileRowsFor(p.pairs, plan->num_experts);
+  while ((1 << p.tile_shift) < p.tile_rows) ++p.tile_shift;
   p.row_tiles = ExpertScaleTiles(p.pairs, plan->num_experts, p.tile_rows);
   p.offsets = plan->offsets;
   p.slots = plan->slots;
@@ -531,22 +589,11 @@ int xse_mxfp4_dequantize(const xse_mx_matrix* q, void* out, int32_t dtype,
   if (out == nullptr) {
     return FailWith(XSE_INVALID_ARGUMENT, "4-bit values: out is null.");
   }
-  const int k_tiles = static_cast<int>(MxKTiles(q->cols));
-  const int row_shift = RowShift((k_tiles + 1) / 2);
-  const int blocks = BlocksForRows(q->rows * q->groups, row_shift);
-  const uint8_t* codes = static_cast<const uint8_t*>(q->codes);
-  const uint8_t* scales = static_cast<const uint8_t*>(q->scales);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == XSE_DT_F32) {
-    DequantizeKernel<float><<<blocks, kThreads, 0, s>>>(
-        codes, scales, q->rows, q->groups, q->cols, MxRowBytes(q->cols),
-        k_tiles, MxRowTiles(q->rows), row_shift, static_cast<float*>(out),
-        group_stride, row_stride);
+    LaunchDequantize<float>(*q, out, group_stride, row_stride, s);
   } else {
-    DequantizeKernel<__nv_bfloat16><<<blocks, kThreads, 0, s>>>(
-        codes, scales, q->rows, q->groups, q->cols, MxRowBytes(q->cols),
-        k_tiles, MxRowTiles(q->rows), row_shift,
-        static_cast<__nv_bfloat16*>(out), group_stride, row_stride);
+    LaunchDequantize<__nv_bfloat16>(*q, out, group_stride, row_stride, s);
   }
   const int rc = LaunchStatus("4-bit dequantisation");
   if (rc == XSE_OK) SetLastLaunchCount(1);

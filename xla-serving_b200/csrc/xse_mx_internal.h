@@ -83,19 +83,8 @@ __device__ __forceinline__ float MxScale(uint32_t s) {
   return s == 255u ? __uint_as_float(0x7fc00000u) : __uint_as_float(s << 23);
 }
 
-// Two E2M1 codes in one byte (lo in the low half): nearest, ties to even,
+// Eight E2M1 codes in one word, element 0 lowest: nearest, ties to even,
 // saturating at 6.
-__device__ __forceinline__ uint32_t MxCodes2(float lo, float hi) {
-  uint32_t r;
-  asm("{\n\t.reg .b8 a;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-      "mov.b32 %0, {a, a, a, a};\n\t}"
-      : "=r"(r)
-      : "f"(lo), "f"(hi));
-  return r & 0xffu;
-}
-
-// Eight codes in one word, element 0 lowest.
 __device__ __forceinline__ uint32_t MxCodes8(const float (&v)[8]) {
   uint32_t r;
   asm("{\n\t.reg .b8 a, b, c, d;\n\t"
@@ -108,14 +97,6 @@ __device__ __forceinline__ uint32_t MxCodes8(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
         "f"(v[6]), "f"(v[7]));
   return r;
-}
-
-// The value of the code in the low four bits: its exponent and fraction bits
-// placed at a float's (a subnormal there for the code 0.5) and rescaled.
-__device__ __forceinline__ float MxCodeValue(uint32_t code) {
-  const float m =
-      __uint_as_float(((code & 8u) << 28) | ((code & 7u) << 22));
-  return m * __uint_as_float(253u << 23);  // 2^126
 }
 
 // Byte offset of the scale of block b of (padded) row r.

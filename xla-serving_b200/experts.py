@@ -96,8 +96,13 @@ def sort(ids, num_experts, plan=None, *, stream=None) -> ExpertPlan:
                                                         num_experts) or \
         plan.device != ids.device:
       raise invalid("the plan has other sizes than ids")
+    size = C.lib.xse_expert_sort_workspace(plan.pairs, num_experts)
+    scratch = torch.empty(size, dtype=torch.uint8, device=ids.device) \
+        if size else None
     C.check(C.lib.xse_expert_sort(ids.data_ptr(), types[ids.dtype],
-                                  ctypes.byref(plan.struct), s))
+                                  ctypes.byref(plan.struct),
+                                  scratch.data_ptr() if size else None, size,
+                                  s))
   return plan
 
 
