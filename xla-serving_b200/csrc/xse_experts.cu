@@ -246,9 +246,10 @@ cudaError_t LaunchSort(const Id* ids, const xse_expert_plan& plan,
   int64_t per_warp = (pairs + blocks * warps - 1) / (blocks * warps);
   per_warp = (per_warp + 31) / 32 * 32;
   const size_t row = sizeof(int) * static_cast<size_t>(plan.num_experts);
-  cudaError_t e = cudaFuncSetAttribute(
-      SortKernel<Id>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      static_cast<int>(sizeof(int) * (kSortWarps + 2) * XSE_MAX_EXPERTS));
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = AllowShared(
+      SortKernel<Id>, sizeof(int) * (kSortWarps + 2) * XSE_MAX_EXPERTS,
+      &allowed);
   if (e != cudaSuccess) return e;
   if (blocks > 1) {
     SortCountKernel<Id><<<blocks, kSortThreads, row, s>>>(
@@ -807,12 +808,13 @@ int Blocks(int64_t work, int per_block, int per_sm) {
 
 template <typename T, int kC>
 cudaError_t LaunchRing(int op, MoveParams p, cudaStream_t s) {
+  static std::atomic<uint64_t> allowed[2] = {};
   const auto kernel = op == kCombine ? CombineRingKernel<T, kC>
                                      : CombineBackwardRingKernel<T, kC>;
   p.row_shift = ThreadShift(p.cols / (16 / static_cast<int>(sizeof(T))),
                             op == kCombine ? 256 : 32);
-  const cudaError_t e = cudaFuncSetAttribute(
-      kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+  const cudaError_t e =
+      AllowShared(kernel, kRingBytes, &allowed[op == kCombine]);
   if (e != cudaSuccess) return e;
   kernel<<<Blocks(p.tokens, kRingThreads >> p.row_shift, 1), kRingThreads,
            kRingBytes, s>>>(p);

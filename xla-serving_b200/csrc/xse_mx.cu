@@ -106,8 +106,7 @@ struct QuantParams {
   int32_t k_tiles;
   int64_t row_bytes;
   int64_t row_tiles;    // scale tiles of a group's rows (of all: with a plan)
-  int32_t tile_rows;    // rows of a product's tile (2^tile_shift)
-  int32_t tile_shift;
+  int32_t tile_rows;    // rows of a product's tile
   uint8_t* codes;
   uint8_t* scales;
   const int32_t* offsets;
@@ -184,7 +183,13 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
                                           int lane, Put put) {
   if constexpr (kMode == kPlain) {
     const int64_t g = p.groups == 1 ? 0 : row / p.rows;
-    put(row, g * p.row_tiles * kMxTileRows + (row - g * p.rows));
+    const int64_t r = row - g * p.rows;
+    if (p.tile_rows == 0) {
+      put(row, g * p.row_tiles * kMxTileRows + r);
+    } else {  // a product's rows: tiles of more than kMxTileRows
+      const uint32_t tile = static_cast<uint32_t>(r) / p.tile_rows;
+      put(row, tile * (2ll * kMxTileRows) + (r - int64_t{tile} * p.tile_rows));
+    }
   } else {
     const int count = kMode == kFromTokens ? p.topk : 1;
     for (int j = 0; j < count; ++j) {
@@ -196,11 +201,10 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
       if (e >= p.num_experts) continue;  // behind the last sorted row
       const int32_t begin = __ldg(p.offsets + e);
       if (begin < 0 || begin > slot) continue;
-      // tile_rows is a power of two; a tile of 256 rows has two scale tiles.
       const int local = slot - begin;
-      const int in_tile = local & (p.tile_rows - 1);
+      const int in_tile = local % p.tile_rows;
       const int64_t tile =
-          ((begin >> p.tile_shift) + e + (local >> p.tile_shift)) *
+          static_cast<int64_t>(begin / p.tile_rows + e + local / p.tile_rows) *
               (p.tile_rows > kMxTileRows ? 2 : 1) + in_tile / kMxTileRows;
       if (tile >= p.row_tiles) continue;
       put(static_cast<int64_t>(slot),
@@ -495,7 +499,8 @@ int RunQuantize(const QuantParams& p, int32_t dtype, int mode,
 
 int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
                  int64_t row_stride, const xse_expert_plan* plan, bool sorted,
-                 void* codes, void* scales, cudaStream_t stream) {
+                 int tile_rows, void* codes, void* scales,
+                 cudaStream_t stream) {
   QuantParams p{};
   p.x = x;
   p.row_stride = row_stride;
@@ -508,11 +513,13 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
   p.row_tiles = MxRowTiles(rows);
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
-  if (plan == nullptr) return RunQuantize(p, dtype, kPlain, stream);
+  if (plan == nullptr) {
+    p.tile_rows = tile_rows > kMxTileRows ? tile_rows : 0;
+    return RunQuantize(p, dtype, kPlain, stream);
+  }
   p.pairs = plan->tokens * plan->topk;
-  p.tile_rows = MxTileRowsFor(p.pairs, plan->num_experts);
-  while ((1 << p.tile_shift) < p.tile_rows) ++p.tile_shift;
-  p.row_tiles = ExpertScaleTiles(p.pairs, plan->num_experts, p.tile_rows);
+  p.tile_rows = tile_rows;
+  p.row_tiles = ExpertScaleTiles(p.pairs, plan->num_experts, tile_rows);
   p.offsets = plan->offsets;
   p.slots = plan->slots;
   p.topk = plan->topk;

@@ -51,7 +51,7 @@ struct Config {
   static constexpr int kBTiles = kN <= 128 ? 1 : 2;  // scale tiles of b
   static constexpr int kStageBytes =
       kABytes + kBBytes + kScaleBytes * (1 + kBTiles);
-  static constexpr int kMost = (204 * 1024) / kStageBytes;
+  static constexpr int kMost = (216 * 1024) / kStageBytes;
   static constexpr int kStages = kMost > 10 ? 10 : kMost;
   // Tensor memory columns: accumulators, then each stage's scales.
   static constexpr int kAccColumns = kN < 32 ? 32 : kN;
@@ -339,29 +339,51 @@ __device__ __forceinline__ void StoreRows(T* y, int64_t stride,
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = Activate(v[i], XSE_ACT_SIGMOID);
   }
+  const bool whole = __all_sync(0xffffffffu, mine) && rows >= 16;
   if constexpr (sizeof(T) == 2) {
     // Two features a store: even lanes take the even rows of a pair of lanes,
-    // odd lanes the odd ones.
+    // odd lanes the odd ones. All exchanges come before the first store.
     if (paired) {
       const bool odd = lane & 1;
+      uint32_t pair[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float got =
+            __shfl_xor_sync(0xffffffffu, odd ? v[2 * i] : v[2 * i + 1], 1);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(
+            odd ? got : v[2 * i], odd ? v[2 * i + 1] : got);
+        __builtin_memcpy(&pair[i], &b, 4);
+      }
       y += odd ? stride - 1 : 0;
       rows -= odd ? 1 : 0;
+      if (whole) {
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float got =
-            __shfl_xor_sync(0xffffffffu, odd ? v[i] : v[i + 1], 1);
-        const float lo = odd ? got : v[i], hi = odd ? v[i + 1] : got;
-        if (mine && i < rows) {
-          *reinterpret_cast<__nv_bfloat162*>(y + i * stride) =
-              __floats2bfloat162_rn(lo, hi);
+        for (int i = 0; i < 8; ++i) {
+          *reinterpret_cast<uint32_t*>(y) = pair[i];
+          y += 2 * stride;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (mine && 2 * i < rows) *reinterpret_cast<uint32_t*>(y) = pair[i];
+          y += 2 * stride;
         }
       }
       return;
     }
   }
+  if (whole) {
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    if (mine && i < rows) Store(y + i * stride, v[i]);
+    for (int i = 0; i < 16; ++i) {
+      Store(y, v[i]);
+      y += stride;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (mine && i < rows) Store(y, v[i]);
+      y += stride;
+    }
   }
 }
 
@@ -740,11 +762,11 @@ int LaunchGemmAs(GemmParams& p, const void* a_codes, const void* b_codes,
     rc = EncodeCodes(&p.b, b_codes, row_bytes, p.rows, 1, 2, kN);
   }
   if (rc != XSE_OK) return rc;
-  const size_t smem = 1024 + C::kStages * C::kStageBytes +
-                      (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
-  cudaError_t e = cudaFuncSetAttribute(
-      MxGemmKernel<kN, T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-      static_cast<int>(smem));
+  constexpr size_t kFixed = 1024 + C::kStages * C::kStageBytes;
+  const size_t smem = kFixed + (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = AllowShared(MxGemmKernel<kN, T>,
+                              kFixed + 8 * (XSE_MAX_EXPERTS + 1), &allowed);
   if (e == cudaSuccess) {
     int64_t blocks = most_items * p.split;
     if (p.split == 1 && blocks > kNumSms) blocks = kNumSms;
@@ -778,10 +800,11 @@ int LaunchGemm(GemmParams& p, int32_t y_dtype, const void* a_codes,
              : LaunchGemmAs<kN, float>(p, a_codes, b_codes, most_items, s);
 }
 
-// The product of rows in b (codes, scales) with w; plan NULL: one group.
+// The product of rows in b (codes, scales) with w in tiles of n rows; plan
+// NULL: one group.
 int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
             int64_t b_tiles, const xse_mx_matrix& w, const float* bias,
-            int32_t activation, const xse_expert_plan* plan, void* y,
+            int32_t activation, const xse_expert_plan* plan, int n, void* y,
             int32_t y_dtype, int64_t y_stride, cudaStream_t s) {
   GemmParams p{};
   p.a_scales = static_cast<const uint8_t*>(w.scales);
@@ -802,8 +825,6 @@ int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
   p.paired = y_dtype == XSE_DT_BF16 && (reinterpret_cast<uintptr_t>(y) & 3) == 0 &&
              y_stride % 2 == 0 && w.rows % 2 == 0;
   p.split = 1;
-  // Rows a group has on average decide the tile's rows.
-  const int n = MxTileRowsFor(rows, p.groups);
   const int64_t row_tiles =
       plan == nullptr ? (rows + n - 1) / n
                       : rows / n + (p.groups < rows ? p.groups : rows);
@@ -824,6 +845,8 @@ int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
       return LaunchGemm<64>(p, y_dtype, w.codes, b_codes, items, s);
     case 128:
       return LaunchGemm<128>(p, y_dtype, w.codes, b_codes, items, s);
+    case 192:
+      return LaunchGemm<192>(p, y_dtype, w.codes, b_codes, items, s);
     default:
       return LaunchGemm<256>(p, y_dtype, w.codes, b_codes, items, s);
   }
@@ -903,17 +926,21 @@ int xse_linear_forward_mxfp4_q(const xse_mx_matrix* x, const xse_mx_matrix* w,
     return FailWith(XSE_INVALID_ARGUMENT,
                     "4-bit layer buffers must be non-null.");
   }
+  // Scale tiles of 128 rows serve tiles of 256.
+  const int n = x->rows > 128 ? 256 : MxTileRowsFor(x->rows, 1, w->cols);
   const int rc =
       RunGemm(x->codes, x->scales, x->rows, MxRowTiles(x->rows), *w, bias,
-              activation, nullptr, y, y_dtype, y_stride,
+              activation, nullptr, n, y, y_dtype, y_stride,
               static_cast<cudaStream_t>(stream));
   if (rc == XSE_OK) SetLastLaunchCount(1);
   return rc;
 }
 
 int64_t xse_linear_mxfp4_workspace(int64_t rows, int32_t in_dim) {
-  return xse_mxfp4_codes_bytes(rows, in_dim, 1) +
-         xse_mxfp4_scales_bytes(rows, in_dim, 1);
+  if (rows < 1 || rows > INT32_MAX || in_dim < 1) return 0;
+  return rows * xse::MxRowBytes(in_dim) +
+         xse::MxProductTiles(rows, xse::MxTileRowsFor(rows, 1, in_dim)) *
+             xse::MxKTiles(in_dim) * xse::kMxTileBytes;
 }
 
 int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
@@ -944,12 +971,13 @@ int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
   }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace);
-  uint8_t* scales = codes + xse_mxfp4_codes_bytes(rows, w->cols, 1);
-  int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, nullptr, false,
+  uint8_t* scales = codes + rows * MxRowBytes(w->cols);
+  const int n = MxTileRowsFor(rows, 1, w->cols);
+  int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, nullptr, false, n,
                         codes, scales, s);
   if (rc == XSE_OK) {
-    rc = RunGemm(codes, scales, rows, MxRowTiles(rows), *w, bias, activation,
-                 nullptr, y, y_dtype, y_stride, s);
+    rc = RunGemm(codes, scales, rows, MxProductTiles(rows, n), *w, bias,
+                 activation, nullptr, n, y, y_dtype, y_stride, s);
   }
   if (rc == XSE_OK) SetLastLaunchCount(2);
   return rc;
@@ -961,7 +989,7 @@ int64_t xse_expert_linear_workspace(int64_t pairs, int32_t num_experts,
       num_experts > XSE_MAX_EXPERTS || in_dim < 1) {
     return 0;
   }
-  const int n = xse::MxTileRowsFor(pairs, num_experts);
+  const int n = xse::MxTileRowsFor(pairs, num_experts, in_dim);
   return pairs * xse::MxRowBytes(in_dim) +
          xse::ExpertScaleTiles(pairs, num_experts, n) *
              xse::MxKTiles(in_dim) * xse::kMxTileBytes;
@@ -1001,13 +1029,13 @@ int xse_expert_linear_mxfp4(const void* x, int32_t x_dtype, int64_t x_stride,
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   uint8_t* codes = static_cast<uint8_t*>(workspace);
   uint8_t* scales = codes + pairs * MxRowBytes(w->cols);
+  const int n = MxTileRowsFor(pairs, plan->num_experts, w->cols);
   int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, plan, sorted != 0,
-                        codes, scales, s);
+                        n, codes, scales, s);
   if (rc == XSE_OK) {
     rc = RunGemm(codes, scales, pairs,
-                 ExpertScaleTiles(pairs, plan->num_experts,
-                                  MxTileRowsFor(pairs, plan->num_experts)),
-                 *w, bias, activation, plan, y, y_dtype, y_stride, s);
+                 ExpertScaleTiles(pairs, plan->num_experts, n), *w, bias,
+                 activation, plan, n, y, y_dtype, y_stride, s);
   }
   if (rc == XSE_OK) SetLastLaunchCount(2);
   return rc;

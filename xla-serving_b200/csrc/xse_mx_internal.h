@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/xse_emb.h"
 #include "../../include/xse_experts.h"
 #include "../../include/xse_mx.h"
@@ -33,6 +35,24 @@ inline bool Aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }
 
+// Lets `kernel` use `bytes` of shared memory on the current device. `done`, a
+// static per kernel, remembers the devices it was set on (the call costs as
+// much as a launch).
+template <typename Kernel>
+cudaError_t AllowShared(Kernel kernel, size_t bytes,
+                        std::atomic<uint64_t>* done) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? uint64_t{1} << device : 0;
+  if ((done->load(std::memory_order_relaxed) & bit) != 0) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel,
+                           cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>(bytes));
+  if (e == cudaSuccess) done->fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 // XSE_OK for a usable matrix of `what`; buffers are checked unless empty.
 int CheckMxMatrix(const xse_mx_matrix* q, const char* what);
 // XSE_OK for a usable plan (arrays non-null where they have entries).
@@ -41,10 +61,21 @@ int CheckExpertPlan(const xse_expert_plan* plan);
 // Rows of a product's tile for groups of rows / groups rows on average. The
 // scales of an expert product's rows are laid out in 512-byte tiles of that
 // many rows each, so that every tile's scales begin a column of tensor memory.
-inline int MxTileRowsFor(int64_t rows, int32_t groups) {
+// 256 rows read the least shared memory per product but leave no room for a
+// second accumulator, which a long k makes up for: 8192 rows to 8192 features,
+// 192 and 256 rows a tile: k 2048 84.6 and 99.5 us, k 4096 143 and 134 us. 128
+// rows: 103 and 180 us.
+inline int MxTileRowsFor(int64_t rows, int32_t groups, int32_t k) {
   const int64_t mean = (rows + groups - 1) / groups;
   if (mean <= 64) return mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-  return groups == 1 && mean > 128 ? 256 : 128;
+  if (mean <= 128) return 128;
+  return groups == 1 && k >= 4096 ? 256 : 192;
+}
+
+// Scale tiles of n-row tiles over `rows` rows of one group: a tile of more
+// than 128 rows has two.
+inline int64_t MxProductTiles(int64_t rows, int n) {
+  return (rows + n - 1) / n * (n > kMxTileRows ? 2 : 1);
 }
 
 // Scale tiles of n rows that hold every expert's rows on tile boundaries:
@@ -55,12 +86,14 @@ inline int64_t ExpertScaleTiles(int64_t pairs, int32_t num_experts, int n) {
   return (pairs / n + num_experts) * (n > kMxTileRows ? 2 : 1);
 }
 
-// Quantises the rows of x for a product: plan NULL as xse_mxfp4_quantize of
-// one contiguous-row group; else to the sorted rows' places (codes by sorted
+// Quantises the rows of x for a product in tiles of `tile_rows`: plan NULL, one
+// group whose scales lie as MxProductTiles says (as xse_mxfp4_quantize lays
+// them out where tile_rows <= 128); else to the sorted rows' places (codes by sorted
 // row, scales as ExpertScaleTiles says), from token rows or sorted ones.
 int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
                  int64_t row_stride, const xse_expert_plan* plan, bool sorted,
-                 void* codes, void* scales, cudaStream_t stream);
+                 int tile_rows, void* codes, void* scales,
+                 cudaStream_t stream);
 
 #ifdef __CUDACC__
 

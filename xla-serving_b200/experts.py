@@ -14,136 +14,169 @@ A mixture of experts for one batch:
 """
 
 import ctypes
-import dataclasses
 
 import torch
 
 from . import _capi as C
-from .mx import (ACT_NONE, MxMatrix, On, check_bias, float_code, invalid,
-                 row_stride)
+from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_stream, elsewhere,
+                 float_code, invalid, layer_output, on, row_stride)
 
 MAX_EXPERTS = 1024
+_INDEX = {torch.int32: C.INDEX_I32, torch.int64: C.INDEX_I64}
 
 
-@dataclasses.dataclass
 class ExpertPlan:
   """(token, choice) pairs sorted by expert (xse_expert_plan), int32:
   offsets [num_experts + 1], order [tokens * topk] (pair of each sorted row,
   -1 behind the last), slots [tokens, topk] (sorted row of each pair, -1 for
   a dropped one)."""
 
-  offsets: torch.Tensor
-  order: torch.Tensor
-  slots: torch.Tensor
+  __slots__ = ("_offsets", "_order", "_slots", "_buffer", "tokens", "topk",
+               "pairs", "num_experts", "ref")
 
-  def __post_init__(self):
-    for name in ("offsets", "order", "slots"):
-      t = getattr(self, name)
+  def __init__(self, offsets, order, slots):
+    for name, t in (("offsets", offsets), ("order", order), ("slots", slots)):
       if t.dtype != torch.int32 or not t.is_cuda or not t.is_contiguous():
         raise invalid(f"plan.{name} must be a contiguous int32 CUDA tensor")
-    if self.slots.dim() != 2 or self.order.numel() != self.slots.numel() or \
-        self.offsets.numel() < 2:
+    if slots.dim() != 2 or order.numel() != slots.numel() or \
+        offsets.numel() < 2:
       raise invalid("a plan has slots [tokens, topk], order [tokens * topk] "
                     "and offsets [num_experts + 1]")
-    if not self.offsets.device == self.order.device == self.slots.device:
+    if not offsets.device == order.device == slots.device:
       raise invalid("a plan's tensors lie on one device")
-    self.struct = C.ExpertPlanStruct(
-        self.offsets.data_ptr(), self.order.data_ptr(), self.slots.data_ptr(),
-        self.tokens, self.topk, self.num_experts)
+    self._offsets, self._order, self._slots = offsets, order, slots
+    self._buffer = slots
+    self._set(offsets.data_ptr(), order.data_ptr(), slots.data_ptr(),
+              *slots.shape, offsets.numel() - 1)
+
+  def _set(self, offsets, order, slots, tokens, topk, num_experts):
+    self.tokens, self.topk, self.num_experts = tokens, topk, num_experts
+    self.pairs = tokens * topk
+    self.ref = ctypes.byref(C.ExpertPlanStruct(offsets, order, slots, tokens,
+                                               topk, num_experts))
+
+  def _view(self, shape, strides, at):
+    return torch.as_strided(self._buffer, shape, strides, at)
 
   @property
-  def tokens(self):
-    return self.slots.shape[0]
+  def slots(self):
+    if self._slots is None:
+      self._slots = self._view((self.tokens, self.topk), (self.topk, 1), 0)
+    return self._slots
 
   @property
-  def topk(self):
-    return self.slots.shape[1]
+  def order(self):
+    if self._order is None:
+      self._order = self._view((self.pairs,), (1,), _quads(self.pairs))
+    return self._order
 
   @property
-  def pairs(self):
-    return self.slots.numel()
-
-  @property
-  def num_experts(self):
-    return self.offsets.numel() - 1
+  def offsets(self):
+    if self._offsets is None:
+      self._offsets = self._view((self.num_experts + 1,), (1,),
+                                 2 * _quads(self.pairs))
+    return self._offsets
 
   @property
   def device(self):
-    return self.slots.device
+    return self._buffer.device
+
+  def get_device(self):
+    return self._buffer.get_device()
 
   @classmethod
   def empty(cls, tokens, topk, num_experts, device="cuda"):
+    """A plan to be filled; its arrays (slots, order, offsets, each on a
+    16-byte boundary) share one allocation."""
     if topk < 1 or not 1 <= num_experts <= MAX_EXPERTS:
       raise invalid(f"an expert plan needs topk >= 1 and 1 to {MAX_EXPERTS} "
                     "experts")
-    new = lambda *shape: torch.empty(shape, dtype=torch.int32, device=device)  # noqa: E731
-    return cls(new(num_experts + 1), new(tokens * topk), new(tokens, topk))
+    part = _quads(tokens * topk)
+    self = cls.__new__(cls)
+    self._buffer = torch.empty(2 * part + num_experts + 1, dtype=torch.int32,
+                               device=device)
+    self._offsets = self._order = self._slots = None
+    start = self._buffer.data_ptr()
+    self._set(start + 8 * part, start + 4 * part, start, tokens, topk,
+              num_experts)
+    return self
+
+
+def _quads(n):
+  """n rounded up to whole 16-byte quads of int32."""
+  return (n + 3) // 4 * 4
 
 
 def sort(ids, num_experts, plan=None, *, stream=None) -> ExpertPlan:
   """The plan of ids [tokens, topk] (int32 or int64): pairs by expert, those
   of one expert in their order. A pair whose id lies outside [0, num_experts)
   is dropped (padding rows are given -1)."""
-  types = {torch.int32: C.INDEX_I32, torch.int64: C.INDEX_I64}
-  if ids.dtype not in types or ids.dim() != 2 or not ids.is_cuda or \
+  code = _INDEX.get(ids.dtype)
+  if code is None or ids.dim() != 2 or not ids.is_cuda or \
       not ids.is_contiguous():
     raise invalid("expert ids must be a contiguous 2-D int32 or int64 CUDA "
                   f"tensor, got {ids.dtype} {tuple(ids.shape)}")
-  with On(ids.device, stream) as s:
-    if plan is None:
-      plan = ExpertPlan.empty(*ids.shape, num_experts, ids.device)
-    elif (plan.tokens, plan.topk, plan.num_experts) != (*ids.shape,
-                                                        num_experts) or \
-        plan.device != ids.device:
-      raise invalid("the plan has other sizes than ids")
-    size = C.lib.xse_expert_sort_workspace(plan.pairs, num_experts)
-    scratch = torch.empty(size, dtype=torch.uint8, device=ids.device) \
-        if size else None
-    C.check(C.lib.xse_expert_sort(ids.data_ptr(), types[ids.dtype],
-                                  ctypes.byref(plan.struct),
-                                  scratch.data_ptr() if size else None, size,
-                                  s))
+  index = ids.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return sort(ids, num_experts, plan)
+  tokens, topk = ids.shape
+  if plan is None:
+    plan = ExpertPlan.empty(tokens, topk, num_experts, ids.device)
+  elif (plan.tokens, plan.topk, plan.num_experts) != (tokens, topk,
+                                                      num_experts):
+    raise invalid("the plan has other sizes than ids")
+  size = C.lib.xse_expert_sort_workspace(plan.pairs, num_experts)
+  scratch = ids.new_empty(size, dtype=torch.uint8) if size else None
+  C.check(C.lib.xse_expert_sort(
+      ids.data_ptr(), code, plan.ref, scratch.data_ptr() if size else None,
+      size, current_stream(index, plan)))
   return plan
 
 
-def _check_rows(t, rows, what):
-  if t.dim() != 2 or t.shape[0] != rows:
+def _rows(t, rows, what):
+  """(columns, row stride) of a tensor with `rows` rows."""
+  stride = row_stride(t, what)
+  if t.shape[0] != rows:
     raise invalid(f"{what} must have {rows} rows, got shape {tuple(t.shape)}")
+  return t.shape[1], stride
 
 
-def _check_weights(weights, plan):
+def _weights(weights, plan):
   if weights is None:
     return None
-  if weights.dtype != torch.float32 or weights.shape != plan.slots.shape or \
+  if weights.dtype != torch.float32 or \
+      weights.shape != (plan.tokens, plan.topk) or \
       not weights.is_contiguous():
     raise invalid("weights must be contiguous float32 of shape "
-                  f"{tuple(plan.slots.shape)}, got {weights.dtype} "
+                  f"{(plan.tokens, plan.topk)}, got {weights.dtype} "
                   f"{tuple(weights.shape)}")
   return weights.data_ptr()
 
 
-def _output(out, rows, like, what="out"):
+def _output(out, rows, cols, like, what="out"):
+  """(tensor, row stride) of an output of `like`'s type."""
   if out is None:
-    return torch.empty((rows, like.shape[1]), dtype=like.dtype,
-                       device=like.device)
-  if tuple(out.shape) != (rows, like.shape[1]) or out.dtype != like.dtype:
-    raise invalid(f"{what} must be {like.dtype} of shape "
-                  f"{(rows, like.shape[1])}, got {out.dtype} "
-                  f"{tuple(out.shape)}")
-  return out
+    return like.new_empty((rows, cols)), cols
+  if out.shape != (rows, cols) or out.dtype != like.dtype:
+    raise invalid(f"{what} must be {like.dtype} of shape {(rows, cols)}, got "
+                  f"{out.dtype} {tuple(out.shape)}")
+  return out, row_stride(out, what)
 
 
 def gather(x, plan: ExpertPlan, out=None, *, stream=None):
   """x's rows in sorted order: out[r] = x[plan.order[r] // topk], zeros behind
   the last sorted row. Its gradient is combine(grad, plan)."""
   code = float_code(x, "x")
-  _check_rows(x, plan.tokens, "x")
-  stride = row_stride(x, "x")
-  with On(plan.device, stream, x, out) as s:
-    out = _output(out, plan.pairs, x)
-    C.check(C.lib.xse_expert_gather(
-        x.data_ptr(), code, x.shape[1], stride, ctypes.byref(plan.struct),
-        out.data_ptr(), row_stride(out, "out"), s))
+  index = x.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return gather(x, plan, out)
+  cols, stride = _rows(x, plan.tokens, "x")
+  out, out_stride = _output(out, plan.pairs, cols, x)
+  C.check(C.lib.xse_expert_gather(
+      x.data_ptr(), code, cols, stride, plan.ref, out.data_ptr(), out_stride,
+      current_stream(index, plan, out)))
   return out
 
 
@@ -152,14 +185,16 @@ def combine(y, plan: ExpertPlan, weights=None, out=None, *, stream=None):
   without them), summed in fp32 in the order of the choices; a row all of
   whose pairs were dropped is zero."""
   code = float_code(y, "y")
-  _check_rows(y, plan.pairs, "y")
-  stride = row_stride(y, "y")
-  w = _check_weights(weights, plan)
-  with On(plan.device, stream, y, weights, out) as s:
-    out = _output(out, plan.tokens, y)
-    C.check(C.lib.xse_expert_combine(
-        y.data_ptr(), code, y.shape[1], stride, ctypes.byref(plan.struct), w,
-        out.data_ptr(), row_stride(out, "out"), s))
+  index = y.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return combine(y, plan, weights, out)
+  cols, stride = _rows(y, plan.pairs, "y")
+  w = _weights(weights, plan)
+  out, out_stride = _output(out, plan.tokens, cols, y)
+  C.check(C.lib.xse_expert_combine(
+      y.data_ptr(), code, cols, stride, plan.ref, w, out.data_ptr(),
+      out_stride, current_stream(index, plan, weights, out)))
   return out
 
 
@@ -170,21 +205,22 @@ def combine_backward(grad, y, plan: ExpertPlan, weights=None, grad_y=None,
   (t, j) the dot product of grad[t] and its sorted row (0 for a dropped
   pair)."""
   code = float_code(y, "y")
-  _check_rows(y, plan.pairs, "y")
-  _check_rows(grad, plan.tokens, "grad")
-  if grad.dtype != y.dtype or grad.shape[1] != y.shape[1]:
+  index = y.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return combine_backward(grad, y, plan, weights, grad_y, grad_weights)
+  cols, y_stride = _rows(y, plan.pairs, "y")
+  grad_cols, grad_stride = _rows(grad, plan.tokens, "grad")
+  if grad.dtype != y.dtype or grad_cols != cols:
     raise invalid("grad and y need one type and width")
-  w = _check_weights(weights, plan)
-  strides = row_stride(grad, "grad"), row_stride(y, "y")
-  with On(plan.device, stream, grad, y, weights, grad_y, grad_weights) as s:
-    grad_y = _output(grad_y, plan.pairs, y, "grad_y")
-    if grad_weights is None:
-      grad_weights = torch.empty(plan.slots.shape, dtype=torch.float32,
-                                 device=plan.device)
-    C.check(C.lib.xse_expert_combine_backward(
-        grad.data_ptr(), y.data_ptr(), code, y.shape[1], *strides,
-        ctypes.byref(plan.struct), w, grad_y.data_ptr(),
-        row_stride(grad_y, "grad_y"), _check_weights(grad_weights, plan), s))
+  w = _weights(weights, plan)
+  grad_y, gy_stride = _output(grad_y, plan.pairs, cols, y, "grad_y")
+  if grad_weights is None:
+    grad_weights = y.new_empty((plan.tokens, plan.topk), dtype=torch.float32)
+  C.check(C.lib.xse_expert_combine_backward(
+      grad.data_ptr(), y.data_ptr(), code, cols, grad_stride, y_stride,
+      plan.ref, w, grad_y.data_ptr(), gy_stride, _weights(grad_weights, plan),
+      current_stream(index, grad, plan, weights, grad_y, grad_weights)))
   return grad_y, grad_weights
 
 
@@ -196,26 +232,21 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
   num_experts groups of [out, in], bias is [num_experts, out]. out is
   [tokens * topk, out] of x's type by default."""
   code = float_code(x, "x")
-  _check_rows(x, plan.pairs if sorted_rows else plan.tokens, "x")
-  if x.shape[1] != w.cols:
-    raise invalid(f"x has {x.shape[1]} columns, w {w.cols}")
-  if w.device != plan.device:
-    raise invalid(f"tensors on {w.device} and {plan.device} in one call")
-  bias_ptr = check_bias(bias, (w.groups, w.rows))
-  stride = row_stride(x, "x")
-  with On(plan.device, stream, x, bias, out) as s:
-    if out is None:
-      out = torch.empty((plan.pairs, w.rows), dtype=x.dtype, device=x.device)
-    elif tuple(out.shape) != (plan.pairs, w.rows):
-      raise invalid(f"out has shape {tuple(out.shape)}, not "
-                    f"{(plan.pairs, w.rows)}")
-    out_code = float_code(out, "out")
-    size = C.lib.xse_expert_linear_workspace(plan.pairs, plan.num_experts,
-                                             w.cols)
-    scratch = torch.empty(size, dtype=torch.uint8, device=plan.device)
-    C.check(C.lib.xse_expert_linear_mxfp4(
-        x.data_ptr(), code, stride, 1 if sorted_rows else 0,
-        ctypes.byref(plan.struct), ctypes.byref(w.struct), bias_ptr,
-        activation, out.data_ptr(), out_code, row_stride(out, "out"),
-        scratch.data_ptr(), size, s))
+  index = x.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return linear(x, plan, w, bias, activation, out,
+                    sorted_rows=sorted_rows)
+  cols, stride = _rows(x, plan.pairs if sorted_rows else plan.tokens, "x")
+  if cols != w.cols:
+    raise invalid(f"x has {cols} columns, w {w.cols}")
+  bias_ptr = bias_pointer(bias, (w.groups, w.rows))
+  out, out_code, out_stride = layer_output(out, x, plan.pairs, w.rows, x.dtype)
+  size = C.lib.xse_expert_linear_workspace(plan.pairs, plan.num_experts, cols)
+  scratch = w.new_empty(size)
+  C.check(C.lib.xse_expert_linear_mxfp4(
+      x.data_ptr(), code, stride, 1 if sorted_rows else 0, plan.ref, w.ref,
+      bias_ptr, activation, out.data_ptr(), out_code, out_stride,
+      scratch.data_ptr(), size,
+      current_stream(index, plan, w, bias, out)))
   return out

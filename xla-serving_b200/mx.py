@@ -8,8 +8,8 @@ dlrm.py. Tensors are torch CUDA tensors; torch is used only for device memory
 and streams.
 """
 
+import contextlib
 import ctypes
-import dataclasses
 from typing import Optional
 
 import torch
@@ -21,6 +21,13 @@ ACT_NONE, ACT_RELU, ACT_SIGMOID = C.ACT_NONE, C.ACT_RELU, C.ACT_SIGMOID
 BLOCK = 32  # elements per scale
 
 _FLOATS = {torch.float32: C.DT_F32, torch.bfloat16: C.DT_BF16}
+
+
+# The current device's index and the raw cudaStream_t of a device's current
+# stream, without building torch objects: a call on a few rows lasts a few
+# microseconds, as long as those would take.
+_current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
+_raw_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
 
 
 def invalid(message):
@@ -39,88 +46,108 @@ def float_code(t, what):
 
 def row_stride(t, what):
   """Row stride of a 2-D tensor whose rows are contiguous."""
-  if t.dim() != 2:
-    raise invalid(f"{what} must be 2-D, got shape {tuple(t.shape)}")
-  rows, cols = t.shape
-  if cols > 1 and t.stride(1) != 1:
+  shape = t.shape
+  if len(shape) != 2:
+    raise invalid(f"{what} must be 2-D, got shape {tuple(shape)}")
+  rows, cols = shape
+  stride, step = t.stride()
+  if cols > 1 and step != 1:
     raise invalid(f"{what} needs unit column stride")
   if rows > 1:
-    if t.stride(0) < cols:
+    if stride < cols:
       raise invalid(f"{what} needs a row stride of at least its columns")
-    return t.stride(0)
+    return stride
   return max(cols, 1)
 
 
-class On:
-  """The device and stream of one call: makes `device` current for the C call
-  and allocates from the given stream's pool. Every tensor of the call must
-  lie on the device."""
-
-  __slots__ = ("device", "stream", "_device", "_stream")
-
-  def __init__(self, device, stream, *tensors):
-    for t in tensors:
-      if t is not None and t.device != device:
-        raise invalid(f"tensors on {t.device} and {device} in one call")
-    if stream is not None and stream.device != device:
-      raise invalid(f"a stream of {stream.device} for tensors on {device}")
-    self.device, self.stream = device, stream
-    self._device = self._stream = None
-
-  def __enter__(self):
-    if torch.cuda.current_device() != self.device.index:
-      self._device = torch.cuda.device(self.device)
-      self._device.__enter__()
-    if self.stream is not None:
-      self._stream = torch.cuda.stream(self.stream)
-      self._stream.__enter__()
-    return stream_handle(self.stream)
-
-  def __exit__(self, *exc):
-    if self._stream is not None:
-      self._stream.__exit__(*exc)
-    if self._device is not None:
-      self._device.__exit__(*exc)
+def elsewhere(index, stream):
+  """Whether a call on device `index` has to change the current device or
+  stream first (it is then made again within `on`)."""
+  return stream is not None or index != _current_device()
 
 
-@dataclasses.dataclass
+@contextlib.contextmanager
+def on(index, stream):
+  """Makes a device and (if given) a stream of it current: the call's scratch
+  and outputs then come from that stream's pool."""
+  if stream is not None and stream.device.index != index:
+    raise invalid(f"a stream of {stream.device} for tensors on device {index}")
+  with torch.cuda.device(index):
+    if stream is None:
+      yield
+    else:
+      with torch.cuda.stream(stream):
+        yield
+
+
+def current_stream(index, *tensors):
+  """cudaStream_t of the current stream of device `index`, on which all the
+  call's tensors must lie."""
+  for t in tensors:
+    if t is not None and t.get_device() != index:
+      raise invalid(f"tensors on {t.device} and device {index} in one call")
+  return _raw_stream(index)
+
+
 class MxMatrix:
-  """`groups` matrices of [rows, cols] in 4 bits (xse_mx_matrix)."""
+  """`groups` matrices of [rows, cols] in 4 bits (xse_mx_matrix): codes and
+  scales are uint8 tensors of xse_mxfp4_codes_bytes and
+  xse_mxfp4_scales_bytes."""
 
-  codes: torch.Tensor   # uint8, xse_mxfp4_codes_bytes
-  scales: torch.Tensor  # uint8, xse_mxfp4_scales_bytes
-  rows: int
-  cols: int
-  groups: int = 1
+  __slots__ = ("_codes", "_scales", "_at", "rows", "cols", "groups", "ref")
 
-  def __post_init__(self):
+  def __init__(self, codes, scales, rows, cols, groups=1):
     for name, t, need in (
-        ("codes", self.codes,
-         C.lib.xse_mxfp4_codes_bytes(self.rows, self.cols, self.groups)),
-        ("scales", self.scales,
-         C.lib.xse_mxfp4_scales_bytes(self.rows, self.cols, self.groups))):
-      if t.dtype != torch.uint8 or not t.is_contiguous() or t.numel() < need:
-        raise invalid(f"4-bit matrix {name}: {need} contiguous uint8 bytes "
-                      f"needed, got {t.numel()} of {t.dtype}")
-    if self.codes.device != self.scales.device:
+        ("codes", codes, C.lib.xse_mxfp4_codes_bytes(rows, cols, groups)),
+        ("scales", scales, C.lib.xse_mxfp4_scales_bytes(rows, cols, groups))):
+      if t.dtype != torch.uint8 or not t.is_contiguous() or \
+          t.numel() < need or not t.is_cuda:
+        raise invalid(f"4-bit matrix {name}: {need} contiguous uint8 bytes on "
+                      f"a CUDA device needed, got {t.numel()} of {t.dtype}")
+    if codes.device != scales.device:
       raise invalid("4-bit matrix: codes and scales on one device")
-    self.struct = C.MxMatrixStruct(self.codes.data_ptr(),
-                                   self.scales.data_ptr(), self.rows,
-                                   self.cols, self.groups)
+    self._codes, self._scales, self._at = codes, scales, None
+    self._set(codes.data_ptr(), scales.data_ptr(), rows, cols, groups)
+
+  def _set(self, codes, scales, rows, cols, groups):
+    self.rows, self.cols, self.groups = rows, cols, groups
+    self.ref = ctypes.byref(C.MxMatrixStruct(codes, scales, rows, cols,
+                                             groups))
+
+  @property
+  def codes(self):
+    return self._codes if self._at is None else self._codes[:self._at]
+
+  @property
+  def scales(self):
+    return self._scales if self._at is None else self._codes[self._at:]
 
   @property
   def device(self):
-    return self.codes.device
+    return self._codes.device
+
+  def get_device(self):
+    return self._codes.get_device()
+
+  def new_empty(self, shape, dtype=torch.uint8):
+    """A tensor on the matrix's device."""
+    return self._codes.new_empty(shape, dtype=dtype)
 
   @classmethod
   def empty(cls, rows, cols, groups=1, device="cuda"):
+    """A matrix to be filled; codes and scales share one allocation."""
     if rows < 0 or rows >= 2 ** 31 or cols < 1 or groups < 1:
       raise invalid("4-bit matrix needs 0 <= rows < 2^31, cols >= 1 and "
                     "groups >= 1.")
-    codes, scales = (
-        torch.empty(f(rows, cols, groups), dtype=torch.uint8, device=device)
-        for f in (C.lib.xse_mxfp4_codes_bytes, C.lib.xse_mxfp4_scales_bytes))
-    return cls(codes, scales, rows, cols, groups)
+    at = groups * rows * ((cols + 31) // 32 * 16)  # a multiple of 16
+    self = cls.__new__(cls)
+    self._codes = torch.empty(
+        at + groups * ((rows + 127) // 128) * ((cols + 127) // 128) * 512,
+        dtype=torch.uint8, device=device)
+    self._scales, self._at = None, at
+    start = self._codes.data_ptr()
+    self._set(start, start + at if start else 0, rows, cols, groups)
+    return self
 
 
 def quantize(x, out: Optional[MxMatrix] = None, *, stream=None) -> MxMatrix:
@@ -128,48 +155,70 @@ def quantize(x, out: Optional[MxMatrix] = None, *, stream=None) -> MxMatrix:
   strides) as an MxMatrix; blocks of 32 run along the last axis. A layer's
   [in, out] kernel is quantised as `quantize(kernel.t())`."""
   code = float_code(x, "x")
-  if x.dim() not in (2, 3):
-    raise invalid(f"x must be 2-D or 3-D, got shape {tuple(x.shape)}")
-  groups = x.shape[0] if x.dim() == 3 else 1
-  rows, cols = x.shape[-2:]
-  with On(x.device, stream, out) as s:
-    if out is None:
-      out = MxMatrix.empty(rows, cols, groups, x.device)
-    elif (out.rows, out.cols, out.groups) != (rows, cols, groups):
-      raise invalid(f"out holds {out.groups} x {out.rows} x {out.cols}, x has "
-                    f"shape {tuple(x.shape)}")
-    C.check(C.lib.xse_mxfp4_quantize(
-        x.data_ptr(), code, x.stride(0) if groups > 1 else 0, x.stride(-2),
-        x.stride(-1), ctypes.byref(out.struct), s))
+  index = x.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return quantize(x, out)
+  shape, strides = x.shape, x.stride()
+  if len(shape) == 2:
+    groups, (rows, cols), group_stride = 1, shape, 0
+  elif len(shape) == 3:
+    groups, rows, cols = shape
+    group_stride = strides[0]
+  else:
+    raise invalid(f"x must be 2-D or 3-D, got shape {tuple(shape)}")
+  if out is None:
+    out = MxMatrix.empty(rows, cols, groups, x.device)
+  elif (out.rows, out.cols, out.groups) != (rows, cols, groups):
+    raise invalid(f"out holds {out.groups} x {out.rows} x {out.cols}, x has "
+                  f"shape {tuple(shape)}")
+  C.check(C.lib.xse_mxfp4_quantize(
+      x.data_ptr(), code, group_stride, strides[-2], strides[-1], out.ref,
+      current_stream(index, out)))
   return out
 
 
 def dequantize(q: MxMatrix, out=None, *, dtype=torch.float32, stream=None):
   """The values q stands for, [rows, cols] ([groups, rows, cols] for several
   groups), in float32 or bfloat16 (exact in both)."""
-  with On(q.device, stream, out) as s:
-    shape = (q.rows, q.cols) if q.groups == 1 else (q.groups, q.rows, q.cols)
-    if out is None:
-      out = torch.empty(shape, dtype=dtype, device=q.device)
-    elif out.shape != shape:
-      raise invalid(f"out has shape {tuple(out.shape)}, not {shape}")
-    code = float_code(out, "out")
-    group = out.stride(0) if q.groups > 1 else 0
-    stride = row_stride(out if q.groups == 1 else out[0], "out")
-    C.check(C.lib.xse_mxfp4_dequantize(ctypes.byref(q.struct), out.data_ptr(),
-                                       code, group, stride, s))
+  index = q.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return dequantize(q, out, dtype=dtype)
+  shape = (q.rows, q.cols) if q.groups == 1 else (q.groups, q.rows, q.cols)
+  if out is None:
+    out = q.new_empty(shape, dtype)
+  elif out.shape != shape:
+    raise invalid(f"out has shape {tuple(out.shape)}, not {shape}")
+  code = float_code(out, "out")
+  if q.groups == 1:
+    group_stride, stride = 0, row_stride(out, "out")
+  else:
+    group_stride, stride = out.stride(0), row_stride(out[0], "out")
+  C.check(C.lib.xse_mxfp4_dequantize(q.ref, out.data_ptr(), code, group_stride,
+                                     stride, current_stream(index, out)))
   return out
 
 
-def check_bias(bias, shape):
+def bias_pointer(bias, shape):
   """Pointer of a float32 bias of `shape`, None without one."""
   if bias is None:
     return None
-  if bias.dtype != torch.float32 or tuple(bias.shape) != shape or \
+  if bias.dtype != torch.float32 or bias.shape != shape or \
       not bias.is_contiguous():
     raise invalid(f"bias must be contiguous float32 of shape {shape}, got "
                   f"{bias.dtype} {tuple(bias.shape)}")
   return bias.data_ptr()
+
+
+def layer_output(out, like, rows, cols, dtype):
+  """(tensor, XSE_DT_*, row stride) of a layer's [rows, cols] output, a new one
+  of `like`'s device without `out`."""
+  if out is None:
+    return like.new_empty((rows, cols), dtype=dtype), _FLOATS[dtype], cols
+  if out.shape != (rows, cols):
+    raise invalid(f"out has shape {tuple(out.shape)}, not {(rows, cols)}")
+  return out, float_code(out, "out"), row_stride(out, "out")
 
 
 def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
@@ -178,35 +227,30 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
   MxMatrix already quantised) and w [out, in]; Q is `quantize`. Accumulated
   in fp32 and rounded once to out's type (x's by default; float32 for an
   MxMatrix)."""
-  quantised = isinstance(x, MxMatrix)
-  if x.device != w.device:
-    raise invalid(f"tensors on {x.device} and {w.device} in one call")
-  with On(w.device, stream, bias, out) as s:
-    rows = x.rows if quantised else x.shape[0]
-    if out is None:
-      out = torch.empty((rows, w.rows), device=w.device,
-                        dtype=torch.float32 if quantised else x.dtype)
-    elif tuple(out.shape) != (rows, w.rows):
-      raise invalid(f"out has shape {tuple(out.shape)}, not "
-                    f"{(rows, w.rows)}")
-    out_code = float_code(out, "out")
-    out_stride = max(row_stride(out, "out"), w.rows)
-    bias_ptr = check_bias(bias, (w.rows,))
-    if quantised:
-      C.check(C.lib.xse_linear_forward_mxfp4_q(
-          ctypes.byref(x.struct), ctypes.byref(w.struct), bias_ptr, activation,
-          out.data_ptr(), out_code, out_stride, s))
-      return out
-    code = float_code(x, "x")
-    stride = row_stride(x, "x")
-    if x.shape[1] != w.cols:
-      raise invalid(f"x has {x.shape[1]} columns, w {w.cols}")
-    size = C.lib.xse_linear_mxfp4_workspace(rows, w.cols)
-    scratch = torch.empty(size, dtype=torch.uint8, device=w.device)
-    C.check(C.lib.xse_linear_forward_mxfp4(
-        x.data_ptr(), code, rows, stride, ctypes.byref(w.struct), bias_ptr,
-        activation, out.data_ptr(), out_code, out_stride, scratch.data_ptr(),
-        size, s))
+  index = w.get_device()
+  if elsewhere(index, stream):
+    with on(index, stream):
+      return linear(x, w, bias, activation, out)
+  bias_ptr = bias_pointer(bias, (w.rows,))
+  if isinstance(x, MxMatrix):
+    out, out_code, out_stride = layer_output(out, w, x.rows, w.rows,
+                                             torch.float32)
+    C.check(C.lib.xse_linear_forward_mxfp4_q(
+        x.ref, w.ref, bias_ptr, activation, out.data_ptr(), out_code,
+        out_stride, current_stream(index, x, bias, out)))
+    return out
+  code = float_code(x, "x")
+  x_stride = row_stride(x, "x")
+  rows, cols = x.shape
+  if cols != w.cols:
+    raise invalid(f"x has {cols} columns, w {w.cols}")
+  out, out_code, out_stride = layer_output(out, x, rows, w.rows, x.dtype)
+  size = C.lib.xse_linear_mxfp4_workspace(rows, cols)
+  scratch = w.new_empty(size)
+  C.check(C.lib.xse_linear_forward_mxfp4(
+      x.data_ptr(), code, rows, x_stride, w.ref, bias_ptr, activation,
+      out.data_ptr(), out_code, out_stride, scratch.data_ptr(), size,
+      current_stream(index, x, bias, out)))
   return out
 
 
