@@ -84,7 +84,8 @@ int xse_expert_combine_backward(const void* grad, const void* y, int32_t dtype,
  * [out, in] and bias [num_experts, out] or NULL. With `sorted` 0, x is
  * [tokens, in] and x_r is row order[r] / topk; with 1, x is
  * [tokens * topk, in] in sorted order (another such layer's output) and rows
- * behind the last are not read. y is [tokens * topk, out]. */
+ * behind the last do not matter. y is [tokens * topk, out]. `workspace` as
+ * xse_linear_forward_mxfp4's. */
 int64_t xse_expert_linear_workspace(int64_t pairs, int32_t num_experts,
                                     int32_t in_dim);
 int xse_expert_linear_mxfp4(const void* x, int32_t x_dtype, int64_t x_stride,

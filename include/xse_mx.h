@@ -76,8 +76,8 @@ int xse_linear_forward_mxfp4_q(const xse_mx_matrix* x, const xse_mx_matrix* w,
 /* The same from unquantised x ([rows, in] of x_dtype, row stride x_stride),
  * which is quantised on the way: equal to xse_mxfp4_quantize followed by
  * xse_linear_forward_mxfp4_q. `workspace` holds
- * xse_linear_mxfp4_workspace(rows, in) bytes, 16-byte aligned, used until the
- * call's work on `stream` is done. */
+ * xse_linear_mxfp4_workspace(rows, in) bytes (none for a few rows: it may then
+ * be NULL), 16-byte aligned, used until the call's work on `stream` is done. */
 int64_t xse_linear_mxfp4_workspace(int64_t rows, int32_t in_dim);
 int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
                              int64_t x_stride, const xse_mx_matrix* w,

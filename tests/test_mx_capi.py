@@ -39,14 +39,15 @@ def test_buffer_sizes(capi):
         groups * rows * blocks * 16
     assert lib.xse_mxfp4_scales_bytes(rows, cols, groups) == \
         groups * tiles * 512
-    assert lib.xse_linear_mxfp4_workspace(rows, cols) >= \
-        rows * blocks * 16 + tiles * 512
+    need = lib.xse_linear_mxfp4_workspace(rows, cols)
+    assert need == 0 if rows <= 32 else need >= rows * blocks * 16 + tiles * 512
   for rows, cols, groups in ((-1, 4, 1), (1, 0, 1), (1, 4, 0), (2 ** 31, 4, 1)):
     assert lib.xse_mxfp4_codes_bytes(rows, cols, groups) == 0
     assert lib.xse_mxfp4_scales_bytes(rows, cols, groups) == 0
   assert lib.xse_expert_linear_workspace(8, 0, 64) == 0
   assert lib.xse_expert_linear_workspace(8, 1025, 64) == 0
-  assert lib.xse_expert_linear_workspace(8, 4, 64) >= 8 * 32 + 512
+  assert lib.xse_expert_linear_workspace(8, 4, 64) == 0
+  assert lib.xse_expert_linear_workspace(800, 4, 64) >= 800 * 32 + 7 * 512
 
 
 def test_expert_scale_tiles_never_overlap():
@@ -108,7 +109,7 @@ def test_matrix_refusals(capi):
 def test_layer_refusals(capi):
   lib = capi.lib
 
-  def layer(x=4096, dtype=0, rows=4, stride=64, w=None, act=0, y=4096,
+  def layer(x=4096, dtype=0, rows=40, stride=64, w=None, act=0, y=4096,
             y_type=0, y_stride=32, scratch=4096, size=1 << 20):
     return lib.xse_linear_forward_mxfp4(
         x, dtype, rows, stride, w or matrix(capi, rows=32), None, act, y,
@@ -126,7 +127,7 @@ def test_layer_refusals(capi):
   refused(capi, layer(y=None), "non-null")
   refused(capi, layer(scratch=None), "non-null")
   refused(capi, layer(scratch=4100), "aligned")
-  refused(capi, layer(size=lib.xse_linear_mxfp4_workspace(4, 64) - 1),
+  refused(capi, layer(size=lib.xse_linear_mxfp4_workspace(40, 64) - 1),
           "workspace")
   assert layer(rows=0, x=None, y=None, scratch=None, size=0) == capi.OK
   two = lib.xse_linear_forward_mxfp4_q
@@ -187,8 +188,8 @@ def test_expert_refusals(capi):
 
   def layer(groups=3, size=1 << 20, flag=0, stride=64):
     return lib.xse_expert_linear_mxfp4(
-        4096, 0, stride, flag, plan(capi), matrix(capi, rows=32,
-                                                  groups=groups),
+        4096, 0, stride, flag, plan(capi, tokens=400),
+        matrix(capi, rows=32, groups=groups),
         None, 0, 4096, 0, 32, 4096, size, None)
 
   refused(capi, layer(groups=2), "one group of w per expert")

@@ -136,36 +136,12 @@ struct Part {
 
   // The scale byte of the block and this lane's codes.
   __device__ uint32_t Quantize(uint32_t (&codes)[kWords]) const {
-    const uint32_t* w = &v[0].x;
-    uint32_t most = 0;
-    if constexpr (sizeof(T) == 2) {
-      // Magnitudes are ordered as 16-bit integers, infinities and NaN last.
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        most = __vmaxu2(most, w[i] & 0x7fff7fffu);
-      }
-      most = max(most & 0xffff0000u, most << 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) most = max(most, w[i] & 0x7fffffffu);
+    uint32_t most = MxLargest<T, 16>(&v[0].x);
+    if constexpr (kLanes == 2) {
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     }
     const uint32_t s = MxScaleByte(most);
-    const float inv = MxInverseScale(s);
-#pragma unroll
-    for (int k = 0; k < kWords; ++k) {
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if constexpr (sizeof(T) == 2) {
-          const uint32_t u = w[4 * k + i / 2];
-          f[i] = __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16) * inv;
-        } else {
-          f[i] = __uint_as_float(w[8 * k + i]) * inv;
-        }
-      }
-      codes[k] = s == 255u ? 0u : MxCodes8(f);
-    }
+    MxEncode<T, kWords>(&v[0].x, s, codes);
     return s;
   }
 };

@@ -18,6 +18,12 @@
 // in memory), warp 1 moves the scales to tensor memory and issues the MMAs,
 // warps 2 to 9 write the results, which overlaps with the next tile's MMAs.
 //
+// Few rows: warps 10 to 17 read and quantise the rows themselves, into a buffer
+// that holds all of a row tile's k. A block takes neighbouring feature tiles,
+// so it does that once for a row tile; a second buffer holds the next one. (In
+// the stages, anew for every feature tile, the rows' latency bounded the
+// kernel: 64 tokens' 4 choices of 64 experts 2048 -> 1024, 23.8 us.)
+//
 // Few tiles: a cluster of `split` blocks shares a tile, each taking a part of
 // k; the parts are added in block order over distributed shared memory.
 //
@@ -26,8 +32,7 @@
 
 #include <cuda.h>
 
-#include <cstring>
-#include <mutex>
+#include <type_traits>
 
 #include "../../include/xse_dlrm.h"
 #include "xse_mx_internal.h"
@@ -38,9 +43,13 @@ namespace {
 constexpr int kM = 128;            // features of a tile
 constexpr int kStageK = 256;       // elements of k per stage (128 bytes)
 constexpr int kEpilogueWarps = 8;  // two per quarter of the lanes
+constexpr int kQuantizeWarps = 8;  // where the product quantises its rows
 constexpr int kThreads = 64 + 32 * kEpilogueWarps;
+constexpr int kThreadsWithRows = kThreads + 32 * kQuantizeWarps;
 constexpr int kABytes = kM * kStageK / 2;
 constexpr int kScaleBytes = 2 * kMxTileBytes;  // a tile row's, per stage
+constexpr int kSharedBytes = 216 * 1024;  // for stages and rows
+constexpr int kMostStages = 10;
 constexpr long long kWaitCycles = 4000000000ll;  // about two seconds
 
 __device__ int g_wait_failed;
@@ -51,8 +60,12 @@ struct Config {
   static constexpr int kBTiles = kN <= 128 ? 1 : 2;  // scale tiles of b
   static constexpr int kStageBytes =
       kABytes + kBBytes + kScaleBytes * (1 + kBTiles);
-  static constexpr int kMost = (216 * 1024) / kStageBytes;
-  static constexpr int kStages = kMost > 10 ? 10 : kMost;
+  static constexpr int kMost = kSharedBytes / kStageBytes;
+  static constexpr int kStages = kMost > kMostStages ? kMostStages : kMost;
+  // Where the product quantises its rows: a stage holds weights alone, and a
+  // buffer of rows kRowStageBytes for every stage of k.
+  static constexpr int kWeightStageBytes = kABytes + kScaleBytes;
+  static constexpr int kRowStageBytes = kBBytes + kScaleBytes;
   // Tensor memory columns: accumulators, then each stage's scales.
   static constexpr int kAccColumns = kN < 32 ? 32 : kN;
   static constexpr int kAccs = kN <= 192 ? 2 : 1;
@@ -72,6 +85,11 @@ struct GemmParams {
   const float* bias;
   void* y;
   const int32_t* offsets;  // expert rows, or NULL for one group of all rows
+  const void* x;           // unquantised rows
+  const int32_t* order;    // x's row of a sorted row is order[row] / topk; NULL
+  int64_t x_stride;        //   for the row itself
+  int32_t topk;
+  int32_t x_aligned;       // rows of x begin on 16-byte boundaries
   int64_t y_stride;
   int64_t rows;            // of b (and y)
   int64_t b_tiles;         // scale tiles of b, of kN rows or more
@@ -84,6 +102,9 @@ struct GemmParams {
   int32_t activation;
   int32_t paired;          // bf16 y: 4-byte aligned pairs of features
   int32_t split;           // blocks of a cluster that share a tile's k
+  int32_t stages;          // of the ring
+  int32_t row_buffers;     // 1 or 2 buffers of quantised rows
+  int32_t row_stages;      // stages of k that one holds
 };
 
 // ---------------------------------------------------------------- PTX forms
@@ -278,13 +299,13 @@ struct Tile {
 
 // Groups' first row tiles (a running count) and rows in shared memory.
 template <int kN>
-__device__ __forceinline__ Tile TileOf(const GemmParams& p, int64_t item,
+__device__ __forceinline__ Tile TileOf(const GemmParams& p, int item,
                                        const int* tile_begin,
                                        const int* row_begin) {
   using C = Config<kN>;
   Tile t;
-  const int64_t n = item / p.m_tiles;
-  t.m = static_cast<int>(item - n * p.m_tiles);
+  const int n = item / p.m_tiles;
+  t.m = item - n * p.m_tiles;
   t.group = 0;
   int64_t at = n;
   int64_t first = 0, count = p.rows;
@@ -387,33 +408,147 @@ __device__ __forceinline__ void StoreRows(T* y, int64_t stride,
   }
 }
 
-template <int kN, typename T>
-__global__ void __launch_bounds__(kThreads, 1)
+// The 32 elements of a block of x in registers.
+template <typename X>
+struct XBlock {
+  static constexpr int kWords = 8 * sizeof(X);
+  uint4 v[kWords / 4];
+
+  // Elements [col, col + 32) of the row at x, zeros from cols on.
+  __device__ void Load(const X* x, int col, int cols, bool aligned) {
+    if (aligned && col + 32 <= cols) {
+#pragma unroll
+      for (int i = 0; i < kWords / 4; ++i) {
+        v[i] = __ldg(reinterpret_cast<const uint4*>(x + col) + i);
+      }
+    } else {
+      uint32_t* w = &v[0].x;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const X e = col + i < cols ? x[col + i] : static_cast<X>(0.0f);
+        if constexpr (sizeof(X) == 2) {
+          const uint32_t bits = __bfloat16_as_ushort(e);
+          w[i / 2] = i % 2 ? w[i / 2] | bits << 16 : bits;
+        } else {
+          w[i] = __float_as_uint(e);
+        }
+      }
+    }
+  }
+};
+
+// One lane's block of a row tile's buffer: `block` counts 32 columns from the
+// first stage of this block's part of k.
+template <int kN, typename X>
+__device__ __forceinline__ void StoreBlock(uint8_t* buffer, int row, int block,
+                                           const XBlock<X>& x) {
+  using C = Config<kN>;
+  const uint32_t* w = &x.v[0].x;
+  const uint32_t s = MxScaleByte(MxLargest<X, XBlock<X>::kWords>(w));
+  uint4 c;
+  MxEncode<X, 4>(w, s, &c.x);
+  uint8_t* codes = buffer + (block >> 3) * C::kRowStageBytes;
+  const int b = block & 7;
+  // The 128-byte swizzle: 16-byte piece b of row r at b ^ (r % 8).
+  *reinterpret_cast<uint4*>(codes + row * 128 + ((b ^ (row & 7)) * 16)) = c;
+  codes[C::kBBytes + (b >> 2) * kMxTileBytes + row * 16 + (b & 3)] =
+      static_cast<uint8_t>(s);
+}
+
+// The row tiles of this block's items, quantised one after another.
+template <int kN, typename X>
+__device__ __forceinline__ void QuantizeTiles(
+    const GemmParams& p, int thread, int first_item, int last_item,
+    int k_begin, int k_end, const int* tile_begin, const int* row_begin,
+    uint8_t* buffers, uint64_t* rows_full_bar, uint64_t* rows_empty_bar,
+    volatile int* failed) {
+  using C = Config<kN>;
+  constexpr int kQuantizeThreads = 32 * kQuantizeWarps;
+  const int blocks = (k_end - k_begin) * 8;
+  int buffer = 0;
+  uint32_t phase = 0;
+  for (int item = first_item; item < last_item;
+       item = (item / p.m_tiles + 1) * p.m_tiles) {
+    const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+    const bool ok = BarrierWait(SharedAddress(rows_empty_bar + buffer),
+                                phase ^ 1, failed);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    uint8_t* to = buffers + buffer * p.row_stages * C::kRowStageBytes;
+    const int total = t.rows * blocks;
+    const auto load = [&](int i, XBlock<X>& x) {
+      const int row = i / blocks, block = i - row * blocks;
+      int64_t r = t.row + row;
+      if (p.order != nullptr) {
+        const int pair = __ldg(p.order + r);
+        r = pair < 0 || pair >= p.rows ? 0 : pair / p.topk;
+      }
+      x.Load(static_cast<const X*>(p.x) + r * p.x_stride,
+             k_begin * kStageK + block * 32, p.k, p.x_aligned);
+    };
+    constexpr int kAtOnce = sizeof(X) == 2 ? 2 : 1;  // registers hold so many
+    for (int i = thread; i < total; i += kAtOnce * kQuantizeThreads) {
+      XBlock<X> x[kAtOnce];
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        if (i + j * kQuantizeThreads < total) load(i + j * kQuantizeThreads, x[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAtOnce; ++j) {
+        const int at = i + j * kQuantizeThreads;
+        if (at < total) StoreBlock<kN, X>(to, at / blocks, at % blocks, x[j]);
+      }
+    }
+    // Generic stores, read by the MMA's proxy.
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+    if ((thread & 31) == 0) BarrierArrive(SharedAddress(rows_full_bar + buffer));
+    if (++buffer == p.row_buffers) {
+      buffer = 0;
+      phase ^= 1;
+    }
+  }
+}
+
+// X: the type of rows that the kernel quantises itself, void where they come
+// as codes and scales.
+template <int kN, typename T, typename X>
+__global__ void
+__launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
     MxGemmKernel(const __grid_constant__ GemmParams p) {
   using C = Config<kN>;
+  constexpr bool kRows = !std::is_void_v<X>;
   extern __shared__ uint8_t raw[];
-  __shared__ alignas(8) uint64_t full_bar[C::kStages];
-  __shared__ alignas(8) uint64_t empty_bar[C::kStages];
+  // Stages' bytes; with rows quantised here, the host gives the ring what the
+  // rows' buffers leave.
+  constexpr int kStageBytes = kRows ? C::kWeightStageBytes : C::kStageBytes;
+  const int num_stages = kRows ? p.stages : C::kStages;
+  __shared__ alignas(8) uint64_t full_bar[kMostStages];
+  __shared__ alignas(8) uint64_t empty_bar[kMostStages];
+  __shared__ alignas(8) uint64_t rows_full_bar[2];
+  __shared__ alignas(8) uint64_t rows_empty_bar[2];
   __shared__ alignas(8) uint64_t acc_full_bar[2];
   __shared__ alignas(8) uint64_t acc_empty_bar[2];
   __shared__ uint32_t tmem_base;
   __shared__ volatile int failed;
-  __shared__ int scan_carry;  // row tiles of all groups
 
   uint8_t* stages = raw + (1024 - (SharedAddress(raw) & 1023)) % 1024;
-  int* tile_begin =
-      reinterpret_cast<int*>(stages + C::kStages * C::kStageBytes);
+  uint8_t* row_buffers = stages + num_stages * kStageBytes;
+  int* tile_begin = reinterpret_cast<int*>(
+      row_buffers +
+      (kRows ? p.row_buffers * p.row_stages * C::kRowStageBytes : 0));
   int* row_begin = tile_begin + (p.groups + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
   const int lane = threadIdx.x & 31;
   const int rank = static_cast<int>(blockIdx.x) % p.split;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kStages; ++i) {
+    for (int i = 0; i < num_stages; ++i) {
       BarrierInit(SharedAddress(full_bar + i), 1);
       BarrierInit(SharedAddress(empty_bar + i), 1);
     }
     for (int i = 0; i < 2; ++i) {
+      BarrierInit(SharedAddress(rows_full_bar + i), kQuantizeWarps);
+      BarrierInit(SharedAddress(rows_empty_bar + i), 1);
       BarrierInit(SharedAddress(acc_full_bar + i), 1);
       BarrierInit(SharedAddress(acc_empty_bar + i), kEpilogueWarps);
     }
@@ -429,44 +564,60 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;"
                  ::: "memory");
   }
-  if (p.offsets != nullptr && warp == 2) {
-    // The plan's offsets, held to [0, rows], and a scan of the row tiles.
-    int carry = 0;
-    for (int base = 0; base <= p.groups; base += 32) {
-      const int i = base + lane;
-      const int rows = static_cast<int>(p.rows);
-      int begin = 0, end = 0;
-      if (i <= p.groups) {
-        begin = min(max(__ldg(p.offsets + i), 0), rows);
-        row_begin[i] = begin;
-      }
-      if (i < p.groups) end = min(max(__ldg(p.offsets + i + 1), 0), rows);
-      int tiles = end > begin && i < p.groups ? (end - begin + kN - 1) / kN : 0;
-      int scan = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, scan, o);
-        if (lane >= o) scan += up;
-      }
-      if (i <= p.groups) tile_begin[i] = carry + scan - tiles;
-      carry += __shfl_sync(0xffffffffu, scan, 31);
+  if (warp == 0 && Elect()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.a) : "memory");
+    if constexpr (!kRows) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&p.b) : "memory");
     }
-    if (lane == 0) scan_carry = carry;
+  }
+  if (p.offsets != nullptr) {
+    // The plan's offsets, held to [0, rows], and a scan of the row tiles.
+    if (warp >= 2) {
+      for (int i = threadIdx.x - 64; i <= p.groups; i += blockDim.x - 64) {
+        row_begin[i] = min(max(__ldg(p.offsets + i), 0),
+                           static_cast<int>(p.rows));
+      }
+    }
+    __syncthreads();
+    if (warp == 2) {
+      int carry = 0;
+      for (int base = 0; base <= p.groups; base += 32) {
+        const int i = base + lane;
+        const int count = i < p.groups ? row_begin[i + 1] - row_begin[i] : 0;
+        const int tiles = count > 0 ? (count + kN - 1) / kN : 0;
+        int scan = tiles;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, scan, o);
+          if (lane >= o) scan += up;
+        }
+        if (i <= p.groups) tile_begin[i] = carry + scan - tiles;
+        carry += __shfl_sync(0xffffffffu, scan, 31);
+      }
+    }
   }
   FenceBeforeSync();
   __syncthreads();
   FenceAfterSync();
   const uint32_t tmem = tmem_base;
-  const int64_t row_tiles =
-      p.offsets != nullptr ? scan_carry : (p.rows + kN - 1) / kN;
-  const int64_t items = row_tiles * p.m_tiles;
-  const int64_t first_item = blockIdx.x / p.split;
-  const int64_t item_step = gridDim.x / p.split;
+  // Fewer than 2^31: y would not fit the memory otherwise.
+  const int row_tiles = p.offsets != nullptr
+                            ? tile_begin[p.groups]
+                            : static_cast<int>((p.rows + kN - 1) / kN);
+  const int items = row_tiles * p.m_tiles;
+  // A block's (a cluster's) items: every item_step-th, or, where it quantises
+  // their rows, neighbouring ones.
+  const int sharers = gridDim.x / p.split, sharer = blockIdx.x / p.split;
+  int first_item = sharer, last_item = items, item_step = sharers;
+  if constexpr (kRows) {
+    const int each = items / sharers, more = items % sharers;
+    first_item = each * sharer + min(sharer, more);
+    last_item = first_item + each + (sharer < more ? 1 : 0);
+    item_step = 1;
+  }
   // This block's part of k, in stages.
-  const int k_begin = static_cast<int>(
-      static_cast<int64_t>(p.k_stages) * rank / p.split);
-  const int k_end = static_cast<int>(
-      static_cast<int64_t>(p.k_stages) * (rank + 1) / p.split);
+  const int k_begin = p.k_stages * rank / p.split;
+  const int k_end = p.k_stages * (rank + 1) / p.split;
   const uint32_t stage_base = SharedAddress(stages);
 
   if (warp == 0) {
@@ -475,14 +626,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;
     bool ok = true;
     int64_t issued = 0;
-    for (int64_t item = first_item; ok && item < items; item += item_step) {
+    for (int item = first_item; ok && item < last_item;
+         item += item_step) {
       const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
       const uint8_t* a_scales =
           p.a_scales + (static_cast<int64_t>(t.group) * p.m_tiles + t.m) *
                            p.k_tiles * kMxTileBytes;
       const uint8_t* b_scales =
           p.b_scales + t.b_tile * p.k_tiles * kMxTileBytes;
-      const bool b_first = t.b_tile < p.b_tiles;
+      const bool b_first = !kRows && t.b_tile < p.b_tiles;
       const bool b_second = C::kBTiles == 2 && t.b_tile + 1 < p.b_tiles;
       for (int s = k_begin; s < k_end; ++s) {
         ok = BarrierWait(SharedAddress(empty_bar + stage), phase ^ 1, &failed);
@@ -490,15 +642,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         if (Elect()) {
           const uint32_t bar = SharedAddress(full_bar + stage);
-          const uint32_t at = stage_base + stage * C::kStageBytes;
-          const uint32_t scales = at + kABytes + C::kBBytes;
+          const uint32_t at = stage_base + stage * kStageBytes;
+          const uint32_t scales = at + kABytes + (kRows ? 0 : C::kBBytes);
           const uint32_t bytes =
               2 * s + 1 < p.k_tiles ? kScaleBytes : kMxTileBytes;
-          BarrierExpect(bar, kABytes + C::kBBytes +
+          BarrierExpect(bar, kABytes + (kRows ? 0 : C::kBBytes) +
                                  bytes * (1 + b_first + b_second));
           TmaLoad3(at, &p.a, s * (kStageK / 2), t.m * kM, t.group, bar);
-          TmaLoad2(at + kABytes, &p.b, s * (kStageK / 2),
-                   static_cast<int>(t.row), bar);
+          if constexpr (!kRows) {
+            TmaLoad2(at + kABytes, &p.b, s * (kStageK / 2),
+                     static_cast<int>(t.row), bar);
+          }
           const int64_t k_at = static_cast<int64_t>(2 * s) * kMxTileBytes;
           BulkLoad(scales, a_scales + k_at, bytes, bar);
           if (b_first) {
@@ -511,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         ++issued;
-        if (++stage == C::kStages) {
+        if (++stage == num_stages) {
           stage = 0;
           phase ^= 1;
         }
@@ -521,24 +675,33 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) {
       volatile int ignored = 0;
       const int in_flight =
-          static_cast<int>(issued < C::kStages ? issued : C::kStages);
+          static_cast<int>(issued < num_stages ? issued : num_stages);
       for (int i = 0; i < in_flight; ++i) {
         if (--stage < 0) {
-          stage = C::kStages - 1;
+          stage = num_stages - 1;
           phase ^= 1;
         }
-        BarrierWait(SharedAddress(full_bar + stage), phase, &ignored);
+        if (!BarrierWait(SharedAddress(full_bar + stage), phase, &ignored)) {
+          break;
+        }
       }
     }
   } else if (warp == 1) {
-    int stage = 0, acc = 0;
-    uint32_t phase = 0, acc_phase = 0;
-    bool ok = true;
-    for (int64_t item = first_item; ok && item < items; item += item_step) {
+    int stage = 0, acc = 0, rows = 0;
+    uint32_t phase = 0, acc_phase = 0, rows_phase = 0;
+    bool new_rows = true, ok = true;
+    for (int item = first_item; ok && item < last_item;
+         item += item_step) {
       ok = BarrierWait(SharedAddress(acc_empty_bar + acc), acc_phase ^ 1,
                        &failed);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
+      if (kRows && new_rows) {
+        ok = BarrierWait(SharedAddress(rows_full_bar + rows), rows_phase,
+                         &failed);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+      }
       const uint32_t d = tmem + acc * C::kAccColumns;
       for (int s = k_begin; s < k_end; ++s) {
         ok = BarrierWait(SharedAddress(full_bar + stage), phase, &failed);
@@ -546,26 +709,34 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         FenceAfterSync();
         if (Elect()) {
-          const uint32_t at = stage_base + stage * C::kStageBytes;
+          const uint32_t at = stage_base + stage * kStageBytes;
+          const uint32_t b_at =
+              kRows ? SharedAddress(row_buffers) +
+                          (rows * p.row_stages + s - k_begin) *
+                              C::kRowStageBytes
+                    : at + kABytes;
           // The stage's own columns: they are free once its last MMAs are
           // done, which the stage's empty barrier has shown.
           const uint32_t a_col =
               tmem + C::kAccs * C::kAccColumns + stage * C::kScaleColumns;
           const uint32_t b_col = a_col + 8;
           const uint64_t a_desc = SwizzledDesc(at);
-          const uint64_t b_desc = SwizzledDesc(at + kABytes);
-          const uint64_t scales = ScaleDesc(at + kABytes + C::kBBytes);
+          const uint64_t b_desc = SwizzledDesc(b_at);
+          const uint64_t a_scales =
+              ScaleDesc(at + kABytes + (kRows ? 0 : C::kBBytes));
+          const uint64_t b_scales =
+              kRows ? ScaleDesc(b_at + C::kBBytes)
+                    : a_scales + kScaleBytes / 16;
           const int left = p.k - s * kStageK;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             if (h * 128 >= left) break;
             // Descriptors count 16 bytes.
-            CopyScales(a_col + h * 4, scales + h * (kMxTileBytes / 16));
+            CopyScales(a_col + h * 4, a_scales + h * (kMxTileBytes / 16));
 #pragma unroll
             for (int q = 0; q < C::kBTiles; ++q) {
               CopyScales(b_col + (h * C::kBTiles + q) * 4,
-                         scales + ((1 + q) * kScaleBytes + h * kMxTileBytes) /
-                                      16);
+                         b_scales + (q * kScaleBytes + h * kMxTileBytes) / 16);
             }
           }
 #pragma unroll
@@ -578,18 +749,35 @@ __global__ void __launch_bounds__(kThreads, 1)
           Commit(SharedAddress(empty_bar + stage));
         }
         __syncwarp();
-        if (++stage == C::kStages) {
+        if (++stage == num_stages) {
           stage = 0;
           phase ^= 1;
         }
       }
       if (!ok) break;
-      if (Elect()) Commit(SharedAddress(acc_full_bar + acc));
+      // The last item of a row tile gives its buffer back.
+      const int then = item + item_step;
+      new_rows = kRows &&
+                 (then >= last_item || then / p.m_tiles != item / p.m_tiles);
+      if (Elect()) {
+        Commit(SharedAddress(acc_full_bar + acc));
+        if (new_rows) Commit(SharedAddress(rows_empty_bar + rows));
+      }
       __syncwarp();
+      if (new_rows && ++rows == p.row_buffers) {
+        rows = 0;
+        rows_phase ^= 1;
+      }
       if (++acc == C::kAccs) {
         acc = 0;
         acc_phase ^= 1;
       }
+    }
+  } else if (kRows && warp >= 2 + kEpilogueWarps) {
+    if constexpr (kRows) {
+      QuantizeTiles<kN, X>(p, threadIdx.x - kThreads, first_item, last_item,
+                           k_begin, k_end, tile_begin, row_begin, row_buffers,
+                           rows_full_bar, rows_empty_bar, &failed);
     }
   } else {
     // Tensor memory lanes [32 q, 32 q + 32) belong to warps with warp % 4 = q.
@@ -600,7 +788,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int first_column = (warp - 2) / 4 * C::kPart;
     int acc = 0;
     uint32_t acc_phase = 0;
-    for (int64_t item = first_item; item < items; item += item_step) {
+    for (int item = first_item; item < last_item; item += item_step) {
       const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
       const int feature = t.m * kM + quarter * 32 + lane;
       const bool mine = feature < p.out;
@@ -667,7 +855,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // One tile per cluster; all its blocks come here, also without a tile.
     __syncwarp();
     ClusterSync();
-    if (warp >= 2 && first_item < items && !failed) {
+    if (warp >= 2 && warp < 2 + kEpilogueWarps && first_item < last_item &&
+        !failed) {
       const Tile t = TileOf<kN>(p, first_item, tile_begin, row_begin);
       const int lane_feature = (warp & 3) * 32 + lane;
       const int feature = t.m * kM + lane_feature;
@@ -752,27 +941,37 @@ int EncodeCodes(CUtensorMap* map, const void* codes, int64_t row_bytes,
   return XSE_OK;
 }
 
-template <int kN, typename T>
+template <int kN, typename T, typename X>
 int LaunchGemmAs(GemmParams& p, const void* a_codes, const void* b_codes,
                  int64_t most_items, cudaStream_t s) {
   using C = Config<kN>;
   const int64_t row_bytes = MxRowBytes(p.k);
   int rc = EncodeCodes(&p.a, a_codes, row_bytes, p.out, p.groups, 3, kM);
-  if (rc == XSE_OK) {
+  if (rc == XSE_OK && std::is_void_v<X>) {
     rc = EncodeCodes(&p.b, b_codes, row_bytes, p.rows, 1, 2, kN);
   }
   if (rc != XSE_OK) return rc;
-  constexpr size_t kFixed = 1024 + C::kStages * C::kStageBytes;
-  const size_t smem = kFixed + (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
+  size_t shared = C::kStages * C::kStageBytes;
+  if constexpr (!std::is_void_v<X>) {
+    p.row_stages = (p.k_stages + p.split - 1) / p.split;
+    const int rows = p.row_stages * C::kRowStageBytes;
+    p.row_buffers = 2 * rows <= kRowBufferBytes ? 2 : 1;
+    p.stages = (kSharedBytes - p.row_buffers * rows) / C::kWeightStageBytes;
+    if (p.stages > kMostStages) p.stages = kMostStages;
+    shared = p.stages * C::kWeightStageBytes + p.row_buffers * rows;
+  }
+  const size_t smem =
+      1024 + shared + (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
   static std::atomic<uint64_t> allowed{0};
-  cudaError_t e = AllowShared(MxGemmKernel<kN, T>,
-                              kFixed + 8 * (XSE_MAX_EXPERTS + 1), &allowed);
+  cudaError_t e =
+      AllowShared(MxGemmKernel<kN, T, X>,
+                  1024 + kSharedBytes + 8 * (XSE_MAX_EXPERTS + 1), &allowed);
   if (e == cudaSuccess) {
     int64_t blocks = most_items * p.split;
     if (p.split == 1 && blocks > kNumSms) blocks = kNumSms;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(blocks));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(std::is_void_v<X> ? kThreads : kThreadsWithRows);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cudaLaunchAttribute attr{};
@@ -781,7 +980,7 @@ int LaunchGemmAs(GemmParams& p, const void* a_codes, const void* b_codes,
     attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, MxGemmKernel<kN, T>, p);
+    e = cudaLaunchKernelEx(&cfg, MxGemmKernel<kN, T, X>, p);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -791,30 +990,59 @@ int LaunchGemmAs(GemmParams& p, const void* a_codes, const void* b_codes,
   return XSE_OK;
 }
 
+// Rows that come quantised.
 template <int kN>
 int LaunchGemm(GemmParams& p, int32_t y_dtype, const void* a_codes,
                const void* b_codes, int64_t most_items, cudaStream_t s) {
   return y_dtype == XSE_DT_BF16
-             ? LaunchGemmAs<kN, __nv_bfloat16>(p, a_codes, b_codes, most_items,
-                                               s)
-             : LaunchGemmAs<kN, float>(p, a_codes, b_codes, most_items, s);
+             ? LaunchGemmAs<kN, __nv_bfloat16, void>(p, a_codes, b_codes,
+                                                     most_items, s)
+             : LaunchGemmAs<kN, float, void>(p, a_codes, b_codes, most_items,
+                                             s);
 }
 
-// The product of rows in b (codes, scales) with w in tiles of n rows; plan
-// NULL: one group.
-int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
-            int64_t b_tiles, const xse_mx_matrix& w, const float* bias,
-            int32_t activation, const xse_expert_plan* plan, int n, void* y,
-            int32_t y_dtype, int64_t y_stride, cudaStream_t s) {
+// Rows that the product quantises.
+template <int kN, typename X>
+int LaunchGemmOfRows(GemmParams& p, int32_t y_dtype, const void* a_codes,
+                     int64_t most_items, cudaStream_t s) {
+  return y_dtype == XSE_DT_BF16
+             ? LaunchGemmAs<kN, __nv_bfloat16, X>(p, a_codes, nullptr,
+                                                  most_items, s)
+             : LaunchGemmAs<kN, float, X>(p, a_codes, nullptr, most_items, s);
+}
+
+// Rows of a product, quantised (codes, scales in tiles of its n rows) or not
+// (x; plan's tokens' rows unless `sorted`).
+struct Rows {
+  const void* codes;
+  const void* scales;
+  int64_t scale_tiles;
+  const void* x;
+  int32_t x_dtype;
+  int64_t x_stride;
+  bool sorted;
+};
+
+// The product of `rows` rows with w in tiles of n rows; plan NULL: one group.
+int RunGemm(const Rows& from, int64_t rows, const xse_mx_matrix& w,
+            const float* bias, int32_t activation, const xse_expert_plan* plan,
+            int n, void* y, int32_t y_dtype, int64_t y_stride,
+            cudaStream_t s) {
   GemmParams p{};
   p.a_scales = static_cast<const uint8_t*>(w.scales);
-  p.b_scales = static_cast<const uint8_t*>(b_scales);
+  p.b_scales = static_cast<const uint8_t*>(from.scales);
+  p.b_tiles = from.scale_tiles;
+  p.x = from.x;
+  p.x_stride = from.x_stride;
+  p.x_aligned = Aligned16(from.x) &&
+                from.x_stride % (from.x_dtype == XSE_DT_BF16 ? 8 : 4) == 0;
   p.bias = bias;
   p.y = y;
   p.offsets = plan != nullptr ? plan->offsets : nullptr;
+  p.order = plan != nullptr && !from.sorted ? plan->order : nullptr;
+  p.topk = plan != nullptr ? plan->topk : 1;
   p.y_stride = y_stride;
   p.rows = rows;
-  p.b_tiles = b_tiles;
   p.groups = plan != nullptr ? plan->num_experts : 1;
   p.out = static_cast<int32_t>(w.rows);
   p.k = w.cols;
@@ -822,8 +1050,9 @@ int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
   p.k_stages = (w.cols + kStageK - 1) / kStageK;
   p.m_tiles = static_cast<int32_t>(MxRowTiles(w.rows));
   p.activation = activation;
-  p.paired = y_dtype == XSE_DT_BF16 && (reinterpret_cast<uintptr_t>(y) & 3) == 0 &&
-             y_stride % 2 == 0 && w.rows % 2 == 0;
+  p.paired = y_dtype == XSE_DT_BF16 &&
+             (reinterpret_cast<uintptr_t>(y) & 3) == 0 && y_stride % 2 == 0 &&
+             w.rows % 2 == 0;
   p.split = 1;
   const int64_t row_tiles =
       plan == nullptr ? (rows + n - 1) / n
@@ -836,19 +1065,30 @@ int RunGemm(const void* b_codes, const void* b_scales, int64_t rows,
       p.split *= 2;
     }
   }
+  if (from.x != nullptr) {
+    const bool half = from.x_dtype == XSE_DT_BF16;
+    if (n == 16) {
+      return half ? LaunchGemmOfRows<16, __nv_bfloat16>(p, y_dtype, w.codes,
+                                                        items, s)
+                  : LaunchGemmOfRows<16, float>(p, y_dtype, w.codes, items, s);
+    }
+    return half ? LaunchGemmOfRows<32, __nv_bfloat16>(p, y_dtype, w.codes,
+                                                      items, s)
+                : LaunchGemmOfRows<32, float>(p, y_dtype, w.codes, items, s);
+  }
   switch (n) {
     case 16:
-      return LaunchGemm<16>(p, y_dtype, w.codes, b_codes, items, s);
+      return LaunchGemm<16>(p, y_dtype, w.codes, from.codes, items, s);
     case 32:
-      return LaunchGemm<32>(p, y_dtype, w.codes, b_codes, items, s);
+      return LaunchGemm<32>(p, y_dtype, w.codes, from.codes, items, s);
     case 64:
-      return LaunchGemm<64>(p, y_dtype, w.codes, b_codes, items, s);
+      return LaunchGemm<64>(p, y_dtype, w.codes, from.codes, items, s);
     case 128:
-      return LaunchGemm<128>(p, y_dtype, w.codes, b_codes, items, s);
+      return LaunchGemm<128>(p, y_dtype, w.codes, from.codes, items, s);
     case 192:
-      return LaunchGemm<192>(p, y_dtype, w.codes, b_codes, items, s);
+      return LaunchGemm<192>(p, y_dtype, w.codes, from.codes, items, s);
     default:
-      return LaunchGemm<256>(p, y_dtype, w.codes, b_codes, items, s);
+      return LaunchGemm<256>(p, y_dtype, w.codes, from.codes, items, s);
   }
 }
 
@@ -888,7 +1128,7 @@ int CheckRowsIn(const void* x, int32_t x_dtype, int64_t rows, int64_t x_stride,
                     "4-bit layer needs 0 <= rows < 2^31 and an input row "
                     "stride >= in.");
   }
-  if (rows > 0 && (x == nullptr || workspace == nullptr)) {
+  if (rows > 0 && (x == nullptr || (need > 0 && workspace == nullptr))) {
     return FailWith(XSE_INVALID_ARGUMENT,
                     "4-bit layer buffers must be non-null.");
   }
@@ -899,6 +1139,35 @@ int CheckRowsIn(const void* x, int32_t x_dtype, int64_t rows, int64_t x_stride,
                     static_cast<long long>(have));
   }
   return XSE_OK;
+}
+
+// A layer over `x_rows` unquantised rows: `rows` products (a sorted row each
+// with a plan) in tiles of n rows.
+int RunLayer(const void* x, int32_t x_dtype, int64_t x_rows, int64_t x_stride,
+             int64_t rows, bool sorted, const xse_expert_plan* plan,
+             int64_t scale_tiles, const xse_mx_matrix& w, const float* bias,
+             int32_t activation, int n, void* y, int32_t y_dtype,
+             int64_t y_stride, void* workspace, cudaStream_t s) {
+  Rows from{};
+  if (MxQuantizesInProduct(n, w.cols)) {
+    from.x = x;
+    from.x_dtype = x_dtype;
+    from.x_stride = x_stride;
+    from.sorted = sorted;
+  } else {
+    uint8_t* codes = static_cast<uint8_t*>(workspace);
+    uint8_t* scales = codes + rows * MxRowBytes(w.cols);
+    const int rc = QuantizeRows(x, x_dtype, x_rows, w.cols, x_stride, plan,
+                                sorted, n, codes, scales, s);
+    if (rc != XSE_OK) return rc;
+    from.codes = codes;
+    from.scales = scales;
+    from.scale_tiles = scale_tiles;
+  }
+  const int rc = RunGemm(from, rows, w, bias, activation, plan, n, y, y_dtype,
+                         y_stride, s);
+  if (rc == XSE_OK) SetLastLaunchCount(from.x != nullptr ? 1 : 2);
+  return rc;
 }
 
 }  // namespace
@@ -928,19 +1197,23 @@ int xse_linear_forward_mxfp4_q(const xse_mx_matrix* x, const xse_mx_matrix* w,
   }
   // Scale tiles of 128 rows serve tiles of 256.
   const int n = x->rows > 128 ? 256 : MxTileRowsFor(x->rows, 1, w->cols);
-  const int rc =
-      RunGemm(x->codes, x->scales, x->rows, MxRowTiles(x->rows), *w, bias,
-              activation, nullptr, n, y, y_dtype, y_stride,
-              static_cast<cudaStream_t>(stream));
+  Rows from{};
+  from.codes = x->codes;
+  from.scales = x->scales;
+  from.scale_tiles = MxRowTiles(x->rows);
+  const int rc = RunGemm(from, x->rows, *w, bias, activation, nullptr, n, y,
+                         y_dtype, y_stride, static_cast<cudaStream_t>(stream));
   if (rc == XSE_OK) SetLastLaunchCount(1);
   return rc;
 }
 
 int64_t xse_linear_mxfp4_workspace(int64_t rows, int32_t in_dim) {
   if (rows < 1 || rows > INT32_MAX || in_dim < 1) return 0;
+  const int n = xse::MxTileRowsFor(rows, 1, in_dim);
+  if (xse::MxQuantizesInProduct(n, in_dim)) return 0;
   return rows * xse::MxRowBytes(in_dim) +
-         xse::MxProductTiles(rows, xse::MxTileRowsFor(rows, 1, in_dim)) *
-             xse::MxKTiles(in_dim) * xse::kMxTileBytes;
+         xse::MxProductTiles(rows, n) * xse::MxKTiles(in_dim) *
+             xse::kMxTileBytes;
 }
 
 int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
@@ -969,18 +1242,10 @@ int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
     return FailWith(XSE_INVALID_ARGUMENT,
                     "4-bit layer buffers must be non-null.");
   }
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  uint8_t* codes = static_cast<uint8_t*>(workspace);
-  uint8_t* scales = codes + rows * MxRowBytes(w->cols);
   const int n = MxTileRowsFor(rows, 1, w->cols);
-  int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, nullptr, false, n,
-                        codes, scales, s);
-  if (rc == XSE_OK) {
-    rc = RunGemm(codes, scales, rows, MxProductTiles(rows, n), *w, bias,
-                 activation, nullptr, n, y, y_dtype, y_stride, s);
-  }
-  if (rc == XSE_OK) SetLastLaunchCount(2);
-  return rc;
+  return RunLayer(x, x_dtype, rows, x_stride, rows, false, nullptr,
+                  MxProductTiles(rows, n), *w, bias, activation, n, y, y_dtype,
+                  y_stride, workspace, static_cast<cudaStream_t>(stream));
 }
 
 int64_t xse_expert_linear_workspace(int64_t pairs, int32_t num_experts,
@@ -990,6 +1255,7 @@ int64_t xse_expert_linear_workspace(int64_t pairs, int32_t num_experts,
     return 0;
   }
   const int n = xse::MxTileRowsFor(pairs, num_experts, in_dim);
+  if (xse::MxQuantizesInProduct(n, in_dim)) return 0;
   return pairs * xse::MxRowBytes(in_dim) +
          xse::ExpertScaleTiles(pairs, num_experts, n) *
              xse::MxKTiles(in_dim) * xse::kMxTileBytes;
@@ -1026,19 +1292,11 @@ int xse_expert_linear_mxfp4(const void* x, int32_t x_dtype, int64_t x_stride,
     return FailWith(XSE_INVALID_ARGUMENT,
                     "4-bit layer buffers must be non-null.");
   }
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  uint8_t* codes = static_cast<uint8_t*>(workspace);
-  uint8_t* scales = codes + pairs * MxRowBytes(w->cols);
   const int n = MxTileRowsFor(pairs, plan->num_experts, w->cols);
-  int rc = QuantizeRows(x, x_dtype, rows, w->cols, x_stride, plan, sorted != 0,
-                        n, codes, scales, s);
-  if (rc == XSE_OK) {
-    rc = RunGemm(codes, scales, pairs,
-                 ExpertScaleTiles(pairs, plan->num_experts, n), *w, bias,
-                 activation, plan, n, y, y_dtype, y_stride, s);
-  }
-  if (rc == XSE_OK) SetLastLaunchCount(2);
-  return rc;
+  return RunLayer(x, x_dtype, rows, x_stride, pairs, sorted != 0, plan,
+                  ExpertScaleTiles(pairs, plan->num_experts, n), *w, bias,
+                  activation, n, y, y_dtype, y_stride, workspace,
+                  static_cast<cudaStream_t>(stream));
 }
 
 int xse_mxfp4_check(void* stream) {

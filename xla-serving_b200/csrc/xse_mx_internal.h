@@ -86,6 +86,18 @@ inline int64_t ExpertScaleTiles(int64_t pairs, int32_t num_experts, int n) {
   return (pairs / n + num_experts) * (n > kMxTileRows ? 2 : 1);
 }
 
+// Whether a product with tiles of n rows quantises its rows itself (then it
+// needs no workspace): each of its blocks reads the rows anew, which for few
+// rows costs less than a launch and a trip through memory. Their k has to fit
+// a buffer of shared memory (n * 128 bytes of codes and 1 KB of scales for
+// every 256 elements).
+constexpr int kRowBufferBytes = 96 * 1024;
+inline bool MxQuantizesInProduct(int n, int32_t k) {
+  return n <= 32 &&
+         (k + 255) / 256 * static_cast<int64_t>(n * 128 + 1024) <=
+             kRowBufferBytes;
+}
+
 // Quantises the rows of x for a product in tiles of `tile_rows`: plan NULL, one
 // group whose scales lie as MxProductTiles says (as xse_mxfp4_quantize lays
 // them out where tile_rows <= 128); else to the sorted rows' places (codes by sorted
@@ -130,6 +142,46 @@ __device__ __forceinline__ uint32_t MxCodes8(const float (&v)[8]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
         "f"(v[6]), "f"(v[7]));
   return r;
+}
+
+// The bits of the largest magnitude among kWords words of T (two bfloat16 or
+// one float a word). Magnitudes are ordered as integers, infinities and NaN
+// last.
+template <typename T, int kWords>
+__device__ __forceinline__ uint32_t MxLargest(const uint32_t* w) {
+  uint32_t most = 0;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      most = __vmaxu2(most, w[i] & 0x7fff7fffu);
+    }
+    return max(most & 0xffff0000u, most << 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) most = max(most, w[i] & 0x7fffffffu);
+    return most;
+  }
+}
+
+// The codes of 8 * kCodeWords elements of a block with scale byte s.
+template <typename T, int kCodeWords>
+__device__ __forceinline__ void MxEncode(const uint32_t* w, uint32_t s,
+                                         uint32_t* codes) {
+  const float inv = MxInverseScale(s);
+#pragma unroll
+  for (int k = 0; k < kCodeWords; ++k) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const uint32_t u = w[4 * k + i / 2];
+        f[i] = __uint_as_float(i % 2 ? u & 0xffff0000u : u << 16) * inv;
+      } else {
+        f[i] = __uint_as_float(w[8 * k + i]) * inv;
+      }
+    }
+    codes[k] = s == 255u ? 0u : MxCodes8(f);
+  }
 }
 
 // Byte offset of the scale of block b of (padded) row r.

@@ -243,10 +243,10 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
   bias_ptr = bias_pointer(bias, (w.groups, w.rows))
   out, out_code, out_stride = layer_output(out, x, plan.pairs, w.rows, x.dtype)
   size = C.lib.xse_expert_linear_workspace(plan.pairs, plan.num_experts, cols)
-  scratch = w.new_empty(size)
+  scratch = w.new_empty(size) if size else None
   C.check(C.lib.xse_expert_linear_mxfp4(
       x.data_ptr(), code, stride, 1 if sorted_rows else 0, plan.ref, w.ref,
       bias_ptr, activation, out.data_ptr(), out_code, out_stride,
-      scratch.data_ptr(), size,
+      scratch.data_ptr() if size else None, size,
       current_stream(index, plan, w, bias, out)))
   return out

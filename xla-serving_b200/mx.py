@@ -246,11 +246,11 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
     raise invalid(f"x has {cols} columns, w {w.cols}")
   out, out_code, out_stride = layer_output(out, x, rows, w.rows, x.dtype)
   size = C.lib.xse_linear_mxfp4_workspace(rows, cols)
-  scratch = w.new_empty(size)
+  scratch = w.new_empty(size) if size else None
   C.check(C.lib.xse_linear_forward_mxfp4(
       x.data_ptr(), code, rows, x_stride, w.ref, bias_ptr, activation,
-      out.data_ptr(), out_code, out_stride, scratch.data_ptr(), size,
-      current_stream(index, x, bias, out)))
+      out.data_ptr(), out_code, out_stride,
+      scratch.data_ptr() if size else None, size, current_stream(index, x, bias, out)))
   return out
 
 
