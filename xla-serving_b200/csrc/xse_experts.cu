@@ -370,9 +370,10 @@ __device__ __forceinline__ void LoadSlots(const MoveParams& p, int64_t t,
 
 // 2^row_shift threads per token, a piece each at a time: the row is read once
 // and stored for all its choices.
-template <typename T, int V>
+template <typename T>
 __global__ void __launch_bounds__(kThreads)
     GatherKernel(const __grid_constant__ MoveParams p) {
+  constexpr int V = 16 / sizeof(T);
   const int per_block = kThreads >> p.row_shift;
   const int mine = threadIdx.x >> p.row_shift;
   const int lane = threadIdx.x & ((1 << p.row_shift) - 1);
@@ -732,60 +733,181 @@ __global__ void __launch_bounds__(kRingThreads, 1)
   if (p.dst != nullptr) ZeroTail<T, 16 / sizeof(T)>(p);
 }
 
-// Rows at any alignment: one element at a time, several tokens per block.
+// Rows at any alignment, one element at a time: a thread has kWide elements of
+// a row (a stride of its group's width apart) and kFew choices in flight, which
+// stand in for the wide loads.
+constexpr int kWide = 4;
+constexpr int kFew = 4;
+
+template <typename T>
+__device__ __forceinline__ void LoadWide(const T* row, int c, int step,
+                                         int cols, float (&v)[kWide]) {
+#pragma unroll
+  for (int i = 0; i < kWide; ++i) {
+    v[i] = c + i * step < cols ? Widen(row[c + i * step]) : 0.0f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void StoreWide(T* row, int c, int step, int cols,
+                                          const float (&v)[kWide]) {
+#pragma unroll
+  for (int i = 0; i < kWide; ++i) {
+    if (c + i * step < cols) row[c + i * step] = Narrow<T>(v[i]);
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    CombineKernel(const __grid_constant__ MoveParams p) {
-  const int per_block = kThreads >> p.row_shift;
-  const int lane = threadIdx.x & ((1 << p.row_shift) - 1);
+    GatherElementsKernel(const __grid_constant__ MoveParams p) {
+  const int per_block = kThreads >> p.row_shift, step = 1 << p.row_shift;
+  const int lane = threadIdx.x & (step - 1);
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * per_block +
                    (threadIdx.x >> p.row_shift);
        t < p.tokens; t += static_cast<int64_t>(gridDim.x) * per_block) {
-    for (int c = lane; c < p.cols; c += 1 << p.row_shift) {
-      float sum = 0.0f;
-#pragma unroll 4
-      for (int j = 0; j < p.topk; ++j) {
-        const int32_t slot = SlotOf(p, t, j);
-        if (slot < 0) continue;
-        const float w = p.weights ? __ldg(p.weights + t * p.topk + j) : 1.0f;
-        sum = fmaf(w, Widen(static_cast<const T*>(p.src)[slot * p.src_stride +
-                                                         c]), sum);
+    const T* x = static_cast<const T*>(p.src) + t * p.src_stride;
+    for (int c = lane; c < p.cols; c += kWide * step) {
+      float v[kWide];
+      LoadWide(x, c, step, p.cols, v);
+      for (int first = 0; first < p.topk; first += kFew) {
+        int32_t slot[kFew];
+        LoadChoices<kFew>(p, p.slots, t, first, -1, slot);
+#pragma unroll
+        for (int j = 0; j < kFew; ++j) {
+          if (!Kept(p, slot[j])) continue;
+          StoreWide(static_cast<T*>(p.dst) + slot[j] * p.dst_stride, c, step,
+                    p.cols, v);
+        }
       }
-      static_cast<T*>(p.dst)[t * p.dst_stride + c] = Narrow<T>(sum);
+    }
+  }
+  ZeroTail<T, 1>(p);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    CombineElementsKernel(const __grid_constant__ MoveParams p) {
+  const int per_block = kThreads >> p.row_shift, step = 1 << p.row_shift;
+  const int lane = threadIdx.x & (step - 1);
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * per_block +
+                   (threadIdx.x >> p.row_shift);
+       t < p.tokens; t += static_cast<int64_t>(gridDim.x) * per_block) {
+    for (int c = lane; c < p.cols; c += kWide * step) {
+      float sum[kWide] = {};
+      for (int first = 0; first < p.topk; first += kFew) {
+        int32_t slot[kFew];
+        float w[kFew], v[kFew][kWide];
+        LoadChoices<kFew>(p, p.slots, t, first, -1, slot);
+        if (p.weights != nullptr) {
+          LoadChoices<kFew>(p, p.weights, t, first, 0.0f, w);
+        }
+#pragma unroll
+        for (int j = 0; j < kFew; ++j) {
+          if (!Kept(p, slot[j])) continue;
+          LoadWide(static_cast<const T*>(p.src) + slot[j] * p.src_stride, c,
+                   step, p.cols, v[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < kFew; ++j) {
+          if (!Kept(p, slot[j])) continue;
+#pragma unroll
+          for (int i = 0; i < kWide; ++i) {
+            sum[i] = fmaf(p.weights ? w[j] : 1.0f, v[j][i], sum[i]);
+          }
+        }
+      }
+      StoreWide(static_cast<T*>(p.dst) + t * p.dst_stride, c, step, p.cols,
+                sum);
     }
   }
 }
 
-// The same for the gradients: one warp per (token, choice).
+// 2^row_shift warps of a block per token and kFew of its choices, each with a
+// part of the row; their parts of a dot product are added in order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    CombineBackwardKernel(const __grid_constant__ MoveParams p) {
-  const int lane = threadIdx.x & 31;
-  const int64_t warps = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) +
-                   threadIdx.x / 32;
-       i < p.pairs; i += warps) {
-    const int64_t t = i / p.topk;
-    const int32_t slot = SlotOf(p, t, static_cast<int>(i - t * p.topk));
-    float dot = 0.0f;
-    if (slot >= 0) {
-      const T* g = static_cast<const T*>(p.src) + t * p.src_stride;
-      const T* y = static_cast<const T*>(p.y) + slot * p.y_stride;
-      T* d = static_cast<T*>(p.dst) + slot * p.dst_stride;
-      const float w = p.weights ? __ldg(p.weights + i) : 1.0f;
-#pragma unroll 4
-      for (int c = lane; c < p.cols; c += 32) {
-        const float a = Widen(g[c]);
-        if (p.grad_weights != nullptr) dot = fmaf(a, Widen(y[c]), dot);
-        if (p.dst != nullptr) d[c] = Narrow<T>(w * a);
+    CombineBackwardElementsKernel(const __grid_constant__ MoveParams p) {
+  __shared__ float parts[kThreads / 32][kFew];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x / 32;
+  const int share = 1 << p.row_shift, part = warp & (share - 1);
+  const int groups = (p.topk + kFew - 1) / kFew;
+  const int64_t units = p.tokens * groups;
+  const int per_block = kThreads / 32 >> p.row_shift;
+  const bool dots = p.grad_weights != nullptr;
+  // All warps of a block take the same steps (they meet at barriers).
+  for (int64_t base = static_cast<int64_t>(blockIdx.x) * per_block;
+       base < units; base += static_cast<int64_t>(gridDim.x) * per_block) {
+    const int64_t u = base + (warp >> p.row_shift);
+    const int64_t t = groups == 1 ? u : u / groups;
+    const int first = static_cast<int>(u - t * groups) * kFew;
+    int32_t slot[kFew];
+    float w[kFew], dot[kFew] = {};
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
+      slot[j] = -1;
+      w[j] = 1.0f;
+    }
+    if (u < units) {
+      LoadChoices<kFew>(p, p.slots, t, first, -1, slot);
+      if (p.weights != nullptr) {
+        LoadChoices<kFew>(p, p.weights, t, first, 0.0f, w);
+      }
+      const T* grad = static_cast<const T*>(p.src) + t * p.src_stride;
+      for (int c = part * 32 * kWide + lane; c < p.cols;
+           c += share * 32 * kWide) {
+        float g[kWide], v[kFew][kWide];
+        LoadWide(grad, c, 32, p.cols, g);
+        if (dots) {
+#pragma unroll
+          for (int j = 0; j < kFew; ++j) {
+            if (!Kept(p, slot[j])) continue;
+            LoadWide(static_cast<const T*>(p.y) + slot[j] * p.y_stride, c, 32,
+                     p.cols, v[j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kFew; ++j) {
+          if (!Kept(p, slot[j])) continue;
+          if (dots) {
+#pragma unroll
+            for (int i = 0; i < kWide; ++i) {
+              dot[j] = fmaf(g[i], v[j][i], dot[j]);
+            }
+          }
+          if (p.dst != nullptr) {
+            float o[kWide];
+#pragma unroll
+            for (int i = 0; i < kWide; ++i) o[i] = w[j] * g[i];
+            StoreWide(static_cast<T*>(p.dst) + slot[j] * p.dst_stride, c, 32,
+                      p.cols, o);
+          }
+        }
       }
     }
-    if (p.grad_weights != nullptr) {
+    if (!dots) continue;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < kFew; ++j) {
 #pragma unroll
       for (int o = 16; o >= 1; o >>= 1) {
-        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], o);
       }
-      if (lane == 0) p.grad_weights[i] = dot;
+      if (lane == 0) parts[warp][j] = dot[j];
+    }
+    if (share > 1) {
+      __syncthreads();
+    } else {
+      __syncwarp();
+    }
+    if (part == 0 && u < units && lane < kFew && first + lane < p.topk) {
+      float sum = 0.0f;
+      for (int k = 0; k < share; ++k) sum += parts[warp + k][lane];
+      p.grad_weights[t * p.topk + first + lane] = sum;
+    }
+    if (share > 1) {
+      __syncthreads();
+    } else {
+      __syncwarp();
     }
   }
   if (p.dst != nullptr) ZeroTail<T, 1>(p);
@@ -824,26 +946,31 @@ cudaError_t LaunchRing(int op, MoveParams p, cudaStream_t s) {
 template <typename T>
 cudaError_t LaunchMove(int op, MoveParams p, bool vec, cudaStream_t s) {
   constexpr int kV = 16 / sizeof(T);
-  if (op == kGather) {
-    p.row_shift = ThreadShift(vec ? p.cols / kV : p.cols, kThreads);
-    const int blocks = Blocks(p.tokens, kThreads >> p.row_shift, 8);
-    if (vec) {
-      GatherKernel<T, kV><<<blocks, kThreads, 0, s>>>(p);
-    } else {
-      GatherKernel<T, 1><<<blocks, kThreads, 0, s>>>(p);
+  if (vec) {
+    if (op != kGather) {
+      return p.topk == 1   ? LaunchRing<T, 1>(op, p, s)
+             : p.topk == 2 ? LaunchRing<T, 2>(op, p, s)
+             : p.topk <= 4 ? LaunchRing<T, 4>(op, p, s)
+                           : LaunchRing<T, 8>(op, p, s);
     }
-  } else if (vec) {
-    return p.topk == 1   ? LaunchRing<T, 1>(op, p, s)
-           : p.topk == 2 ? LaunchRing<T, 2>(op, p, s)
-           : p.topk <= 4 ? LaunchRing<T, 4>(op, p, s)
-                         : LaunchRing<T, 8>(op, p, s);
-  } else if (op == kCombine) {
-    p.row_shift = ThreadShift(p.cols, kThreads);
-    CombineKernel<T><<<Blocks(p.tokens, kThreads >> p.row_shift, 8), kThreads,
-                       0, s>>>(p);
+    p.row_shift = ThreadShift(p.cols / kV, kThreads);
+    GatherKernel<T><<<Blocks(p.tokens, kThreads >> p.row_shift, 8), kThreads,
+                      0, s>>>(p);
+  } else if (op == kBackward) {
+    p.row_shift =
+        ThreadShift((p.cols + 32 * kWide - 1) / (32 * kWide), kThreads / 32);
+    CombineBackwardElementsKernel<T>
+        <<<Blocks(p.tokens * ((p.topk + kFew - 1) / kFew),
+                  kThreads / 32 >> p.row_shift, 8),
+           kThreads, 0, s>>>(p);
   } else {
-    CombineBackwardKernel<T>
-        <<<Blocks(p.pairs, kThreads / 32, 8), kThreads, 0, s>>>(p);
+    p.row_shift = ThreadShift((p.cols + kWide - 1) / kWide, kThreads);
+    const int blocks = Blocks(p.tokens, kThreads >> p.row_shift, 8);
+    if (op == kGather) {
+      GatherElementsKernel<T><<<blocks, kThreads, 0, s>>>(p);
+    } else {
+      CombineElementsKernel<T><<<blocks, kThreads, 0, s>>>(p);
+    }
   }
   return cudaGetLastError();
 }

@@ -125,18 +125,19 @@ __device__ __forceinline__ float ToFloat(__nv_bfloat16 v) {
   return __bfloat162float(v);
 }
 
-// The 64 bytes of a row that a lane quantises: a whole block of bfloat16, half
-// a block of float32 (two lanes then agree on the scale).
-template <typename T>
+// The kBytes of a row that a lane quantises: a block or half of one (two lanes
+// then agree on the scale).
+template <typename T, int kBytes>
 struct Part {
-  static constexpr int kElements = 64 / sizeof(T);
+  static constexpr int kElements = kBytes / sizeof(T);
   static constexpr int kLanes = kMxBlock / kElements;  // of a block
   static constexpr int kWords = kElements / 8;         // of codes
-  uint4 v[4];
+  static constexpr int kPieces = kBytes / 16;
+  uint4 v[kPieces];
 
   // The scale byte of the block and this lane's codes.
   __device__ uint32_t Quantize(uint32_t (&codes)[kWords]) const {
-    uint32_t most = MxLargest<T, 16>(&v[0].x);
+    uint32_t most = MxLargest<T, kBytes / 4>(&v[0].x);
     if constexpr (kLanes == 2) {
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     }
@@ -191,16 +192,20 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
 
 // A warp takes 32 parts of a row at a time. kAligned: a lane's 64 bytes are
 // loaded as they lie, four 16-byte loads that share cache lines with the
-// neighbouring lanes' (any split that keeps the loads contiguous over the warp
-// needs shuffles for the blocks' magnitudes and, worse, one scale per 8
-// elements: 31 us against KA us for 8192 x 4096 bf16). Otherwise the elements
-// are loaded one by one over the warp and turned through shared memory.
+// neighbouring lanes' (with loads contiguous over the warp, four or more lanes
+// share a block's scale and its arithmetic is repeated in each: 31 us against
+// 16 us for 8192 x 4096 bf16). Otherwise the elements are loaded one by one
+// over the warp and turned through shared memory.
+template <typename T, bool kAligned>
+using PartOf = Part<T, kAligned || sizeof(T) == 4 ? 64 : 32>;
+
 template <typename T, int kMode, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     QuantizeKernel(const __grid_constant__ QuantParams p) {
-  using P = Part<T>;
+  using P = PartOf<T, kAligned>;
   constexpr int kSpan = 32 * P::kElements;
-  __shared__ uint4 turn[kAligned ? 1 : kThreads / 32][kAligned ? 1 : 128];
+  __shared__ uint4 turn[kAligned ? 1 : kThreads / 32]
+                       [kAligned ? 1 : 32 * P::kPieces];
   const int lane = threadIdx.x & 31;
   const int padded = p.k_tiles * 128, code_cols = (p.cols + 31) / 32 * 32;
   const WarpRow w = FirstRow(p.row_shift);
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__(kThreads)
         const uint4* src = reinterpret_cast<const uint4*>(x + col);
         if (col + P::kElements <= p.cols) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) part.v[i] = __ldg(src + i);
+          for (int i = 0; i < P::kPieces; ++i) part.v[i] = __ldg(src + i);
         } else {
           T* e = reinterpret_cast<T*>(part.v);
 #pragma unroll
@@ -223,10 +228,13 @@ __global__ void __launch_bounds__(kThreads)
           }
         }
       } else {
-        // 16-byte piece c lies at c ^ (c / 8 % 4), so that neither the stores
-        // nor the lanes' loads meet in a bank.
+        // 16-byte piece c lies where neither the stores nor the lanes' loads
+        // meet in a bank.
         T* mine = reinterpret_cast<T*>(turn[threadIdx.x / 32]);
         constexpr int kPiece = 16 / sizeof(T);
+        const auto place = [](int c) {
+          return P::kPieces == 4 ? c ^ (c >> 3 & 3) : c ^ (c >> 3 & 1);
+        };
         T v[P::kElements];
 #pragma unroll
         for (int i = 0; i < P::kElements; ++i) {
@@ -236,18 +244,18 @@ __global__ void __launch_bounds__(kThreads)
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < P::kElements; ++i) {
-          const int e = 32 * i + lane, piece = e / kPiece;
-          mine[(piece ^ (piece >> 3 & 3)) * kPiece + e % kPiece] = v[i];
+          const int e = 32 * i + lane;
+          mine[place(e / kPiece) * kPiece + e % kPiece] = v[i];
         }
         __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int piece = lane * 4 + i;
-          part.v[i] = turn[threadIdx.x / 32][piece ^ (piece >> 3 & 3)];
+        for (int i = 0; i < P::kPieces; ++i) {
+          part.v[i] = turn[threadIdx.x / 32][place(lane * P::kPieces + i)];
         }
       }
       uint32_t codes[P::kWords];
       uint32_t scales = part.Quantize(codes);
+      if (col >= code_cols) scales = 0;  // blocks past the last
       // The scale bytes of four blocks as one word.
       scales |= __shfl_down_sync(0xffffffffu, scales, P::kLanes) << 8;
       scales |= __shfl_down_sync(0xffffffffu, scales, 2 * P::kLanes) << 16;
@@ -326,18 +334,39 @@ __device__ __forceinline__ void DecodeCodes(uint32_t word, uint32_t (&v)[4]) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T FromFloat(float v);
-template <>
-__device__ __forceinline__ float FromFloat(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 FromFloat(float v) {
-  return __float2bfloat16_rn(v);
+// Pairs of bfloat16 times a power of two (or NaN), as eight values of T. The
+// products are exact in bfloat16, whose multiplication keeps subnormals.
+__device__ __forceinline__ void ScaleValues(const uint32_t (&v)[4], uint32_t s,
+                                            uint4 (&out)[1], __nv_bfloat16) {
+  const uint32_t bits = __float_as_uint(MxScale(s)) >> 16;
+  const uint32_t pair = bits << 16 | bits;
+  __nv_bfloat162 m;
+  __builtin_memcpy(&m, &pair, 4);
+  uint32_t* o = &out[0].x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    __nv_bfloat162 a;
+    __builtin_memcpy(&a, &v[i], 4);
+    a = __hmul2(a, m);
+    __builtin_memcpy(&o[i], &a, 4);
+  }
+}
+__device__ __forceinline__ void ScaleValues(const uint32_t (&v)[4], uint32_t s,
+                                            uint4 (&out)[2], float) {
+  const float scale = MxScale(s);
+  uint32_t* o = &out[0].x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    o[2 * i] = __float_as_uint(__uint_as_float(v[i] << 16) * scale);
+    o[2 * i + 1] =
+        __float_as_uint(__uint_as_float(v[i] & 0xffff0000u) * scale);
+  }
 }
 
-// A warp takes 256 columns of a row, a lane eight of one block. kAligned: it
-// stores them whole; otherwise they are turned through shared memory, so that
-// the warp stores neighbouring elements.
+// A warp takes 512 columns of a row, a lane eight of one block of each half.
+// Values go through shared memory, so that the warp stores whole sectors: 16
+// bytes a lane where rows are aligned, else single elements (a lane's own 32
+// bytes of float32 stored as two halves: 42 us against 29 us for 8192 x 4096).
 template <typename T, bool kAligned>
 __global__ void __launch_bounds__(kThreads)
     DequantizeKernel(const uint8_t* __restrict__ codes,
@@ -346,9 +375,12 @@ __global__ void __launch_bounds__(kThreads)
                      int64_t row_tiles, int row_shift, T* __restrict__ out,
                      int64_t group_stride, int64_t row_stride) {
   constexpr int kPiece = 16 / sizeof(T), kPieces = 8 / kPiece;
-  __shared__ uint4 turn[kAligned ? 1 : kThreads / 32]
-                       [kAligned ? 1 : 32 * kPieces];
+  __shared__ uint4 turn[kThreads / 32][32 * kPieces];
   const int lane = threadIdx.x & 31;
+  uint4* mine = turn[threadIdx.x / 32];
+  // Piece c lies at c ^ (c / 8 % 2): two pieces of a lane, 32 bytes apart from
+  // the next lane's, then meet in no bank.
+  const auto place = [](int c) { return kPieces == 2 ? c ^ (c >> 3 & 1) : c; };
   const int padded = k_tiles * 128;
   const WarpRow w = FirstRow(row_shift);
   for (int64_t row = w.row; row < rows * groups; row += w.step) {
@@ -357,56 +389,51 @@ __global__ void __launch_bounds__(kThreads)
     T* o = out + g * group_stride + r * row_stride;
     const uint8_t* row_scales =
         scales + MxScaleAt(g * row_tiles * kMxTileRows + r, 0, k_tiles);
-    for (int first = w.chunk * 256; first < padded; first += w.chunks * 256) {
-      const int col = first + lane * 8;
-      uint32_t word = 0, s = 0;
-      if (col < cols) {
-        word = __ldg(reinterpret_cast<const uint32_t*>(
-            codes + row * row_bytes + col / 2));
-        s = __ldg(row_scales + col / 128 * kMxTileBytes + col / 32 % 4);
-      }
-      const float scale = MxScale(s);
-      uint32_t v[4];
-      DecodeCodes(word, v);
-      alignas(16) T e[8];
+    for (int span = w.chunk * 512; span < padded; span += w.chunks * 512) {
+      uint32_t word[2] = {}, s[2] = {};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        e[2 * i] = FromFloat<T>(__uint_as_float(v[i] << 16) * scale);
-        e[2 * i + 1] =
-            FromFloat<T>(__uint_as_float(v[i] & 0xffff0000u) * scale);
+      for (int h = 0; h < 2; ++h) {
+        const int col = span + h * 256 + lane * 8;
+        if (col < cols) {
+          word[h] = __ldg(reinterpret_cast<const uint32_t*>(
+              codes + row * row_bytes + col / 2));
+          s[h] = __ldg(row_scales + col / 128 * kMxTileBytes + col / 32 % 4);
+        }
       }
-      const uint4* pieces = reinterpret_cast<const uint4*>(e);
-      if constexpr (kAligned) {
-        if (col + 8 <= cols) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int first = span + h * 256;
+        if (first >= cols) break;
+        uint32_t v[4];
+        uint4 pieces[kPieces];
+        DecodeCodes(word[h], v);
+        ScaleValues(v, s[h], pieces, T());
+        if (kAligned && kPieces == 1 && first + 256 <= cols) {
+          reinterpret_cast<uint4*>(o + first)[lane] = pieces[0];
+          continue;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < kPieces; ++i) {
+          mine[place(lane * kPieces + i)] = pieces[i];
+        }
+        __syncwarp();
+        const T* values = reinterpret_cast<const T*>(mine);
+        if (kAligned && first + 256 <= cols) {
 #pragma unroll
           for (int i = 0; i < kPieces; ++i) {
-            reinterpret_cast<uint4*>(o + col)[i] = pieces[i];
+            const int c = 32 * i + lane;
+            reinterpret_cast<uint4*>(o + first)[c] = mine[place(c)];
           }
         } else {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            if (col + i < cols) o[col + i] = e[i];
+            const int at = 32 * i + lane;
+            if (first + at < cols) {
+              o[first + at] =
+                  values[place(at / kPiece) * kPiece + at % kPiece];
+            }
           }
-        }
-      } else {
-        // Piece c lies at c ^ (c / 8 % 2): two pieces of a lane, 32 bytes
-        // apart from the next lane's, then meet in no bank.
-        uint4* mine = turn[threadIdx.x / 32];
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-          const int c = lane * kPieces + i;
-          mine[kPieces == 2 ? c ^ (c >> 3 & 1) : c] = pieces[i];
-        }
-        __syncwarp();
-        const T* values = reinterpret_cast<const T*>(mine);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int at = 32 * i + lane, c = at / kPiece;
-          const T value =
-              values[(kPieces == 2 ? c ^ (c >> 3 & 1) : c) * kPiece +
-                     at % kPiece];
-          if (first + at < cols) o[first + at] = value;
         }
       }
     }
@@ -419,15 +446,20 @@ int BlocksFor(int64_t work, int per_block) {
   return static_cast<int>(b < 1 ? 1 : (b > most ? most : b));
 }
 
-template <typename T, int kMode>
-void LaunchQuantize(QuantParams p, bool aligned, cudaStream_t s) {
-  constexpr int kSpan = 32 * Part<T>::kElements;
+template <typename T, int kMode, bool kAligned>
+void LaunchQuantizeRows(QuantParams p, cudaStream_t s) {
+  constexpr int kSpan = 32 * PartOf<T, kAligned>::kElements;
   p.row_shift = RowShift((p.k_tiles * 128 + kSpan - 1) / kSpan);
-  const int blocks = BlocksForRows(p.total_rows, p.row_shift);
+  QuantizeKernel<T, kMode, kAligned>
+      <<<BlocksForRows(p.total_rows, p.row_shift), kThreads, 0, s>>>(p);
+}
+
+template <typename T, int kMode>
+void LaunchQuantize(const QuantParams& p, bool aligned, cudaStream_t s) {
   if (aligned) {
-    QuantizeKernel<T, kMode, true><<<blocks, kThreads, 0, s>>>(p);
+    LaunchQuantizeRows<T, kMode, true>(p, s);
   } else {
-    QuantizeKernel<T, kMode, false><<<blocks, kThreads, 0, s>>>(p);
+    LaunchQuantizeRows<T, kMode, false>(p, s);
   }
 }
 
@@ -435,7 +467,7 @@ template <typename T>
 void LaunchDequantize(const xse_mx_matrix& q, void* out, int64_t group_stride,
                       int64_t row_stride, cudaStream_t s) {
   const int k_tiles = static_cast<int>(MxKTiles(q.cols));
-  const int row_shift = RowShift((k_tiles + 1) / 2);
+  const int row_shift = RowShift((k_tiles + 3) / 4);
   const int64_t per = 16 / sizeof(T);
   const bool aligned = Aligned16(out) && row_stride % per == 0 &&
                        (q.groups == 1 || group_stride % per == 0);
