@@ -62,7 +62,7 @@ def activate(y, act):
   if act == 1:
     return np.where(y < 0, 0.0, y)
   if act == 2:
-    return 1.0 / (1.0 + np.exp(-y))
+    return 1.0 / (1.0 + np.exp(-np.clip(y, -700.0, 700.0)))
   return y
 
 

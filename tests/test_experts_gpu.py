@@ -202,7 +202,8 @@ def test_strided_rows(experts):
 LAYERS = [  # tokens, topk, experts, in, out
     (1, 1, 1, 32, 16), (4, 2, 8, 64, 128), (64, 4, 16, 256, 200),
     (40, 2, 3, 479, 64), (300, 4, 4, 512, 256), (200, 8, 64, 100, 130),
-    (1500, 2, 6, 320, 128), (2, 1, 256, 700, 40), (600, 1, 1, 96, 96)]
+    (1500, 2, 6, 320, 128), (2, 1, 256, 700, 40), (600, 1, 1, 96, 96),
+    (900, 2, 5, 1600, 270), (700, 1, 2, 2048, 128), (30, 2, 40, 9000, 140)]
 
 
 def expert_reference(x_rows, offsets, w, bias, act):
@@ -250,13 +251,15 @@ def test_linear(mx, experts, tokens, topk, num_experts, cols, out, dtype):
   mx.check()
 
 
-def test_linear_with_even_and_extreme_groups(mx, experts):
+@pytest.mark.parametrize("cols", [128, 1536])
+def test_linear_with_even_and_extreme_groups(mx, experts, cols):
   """All rows in one expert, none at all, and counts around a tile's rows."""
-  num_experts, cols, out = 8, 128, 96
+  num_experts, out = 8, 96
   w, values = expert_weights(mx, num_experts, out, cols)
   for counts in ([0, 0, 0, 500, 0, 0, 0, 0], [0] * 8,
                  [127, 128, 129, 1, 0, 255, 256, 257],
-                 [15, 16, 17, 1, 0, 31, 32, 33], [1] * 8):
+                 [15, 16, 17, 1, 0, 31, 32, 33], [1] * 8,
+                 [255, 256, 257, 1, 0, 511, 512, 600]):
     ids = np.repeat(np.arange(8), counts)[:, None]
     ids = np.concatenate([ids, np.full((3, 1), -1)])
     np.random.default_rng(1).shuffle(ids)

@@ -156,7 +156,9 @@ LAYERS = [  # rows, in, out
     (1, 1, 1), (1, 32, 128), (3, 64, 7), (16, 256, 130), (17, 257, 128),
     (5, 13, 512), (33, 100, 64), (64, 320, 200), (65, 128, 129),
     (100, 479, 1024), (128, 512, 256), (300, 96, 333), (1, 4096, 1024),
-    (20, 3000, 140), (700, 600, 512), (2, 2048, 4096)]
+    (20, 3000, 140), (700, 600, 512), (2, 2048, 4096), (257, 1536, 128),
+    (700, 1700, 390), (129, 2048, 7), (513, 2100, 1000), (40, 9000, 130),
+    (8, 9000, 33)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

@@ -160,13 +160,7 @@ __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
                                           int lane, Put put) {
   if constexpr (kMode == kPlain) {
     const int64_t g = p.groups == 1 ? 0 : row / p.rows;
-    const int64_t r = row - g * p.rows;
-    if (p.tile_rows == 0) {
-      put(row, g * p.row_tiles * kMxTileRows + r);
-    } else {  // a product's rows: tiles of more than kMxTileRows
-      const uint32_t tile = static_cast<uint32_t>(r) / p.tile_rows;
-      put(row, tile * (2ll * kMxTileRows) + (r - int64_t{tile} * p.tile_rows));
-    }
+    put(row, g * p.row_tiles * kMxTileRows + (row - g * p.rows));
   } else {
     const int count = kMode == kFromTokens ? p.topk : 1;
     for (int j = 0; j < count; ++j) {
@@ -521,10 +515,7 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
   p.row_tiles = MxRowTiles(rows);
   p.codes = static_cast<uint8_t*>(codes);
   p.scales = static_cast<uint8_t*>(scales);
-  if (plan == nullptr) {
-    p.tile_rows = tile_rows > kMxTileRows ? tile_rows : 0;
-    return RunQuantize(p, dtype, kPlain, stream);
-  }
+  if (plan == nullptr) return RunQuantize(p, dtype, kPlain, stream);
   p.pairs = plan->tokens * plan->topk;
   p.tile_rows = tile_rows;
   p.row_tiles = ExpertScaleTiles(p.pairs, plan->num_experts, tile_rows);

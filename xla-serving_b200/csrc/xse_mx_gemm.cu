@@ -57,9 +57,8 @@ __device__ int g_wait_failed;
 template <int kN>
 struct Config {
   static constexpr int kBBytes = kN * kStageK / 2;
-  static constexpr int kBTiles = kN <= 128 ? 1 : 2;  // scale tiles of b
-  static constexpr int kStageBytes =
-      kABytes + kBBytes + kScaleBytes * (1 + kBTiles);
+  static_assert(kN <= kMxTileRows, "one scale tile of b");
+  static constexpr int kStageBytes = kABytes + kBBytes + 2 * kScaleBytes;
   static constexpr int kMost = kSharedBytes / kStageBytes;
   static constexpr int kStages = kMost > kMostStages ? kMostStages : kMost;
   // Where the product quantises its rows: a stage holds weights alone, and a
@@ -68,8 +67,8 @@ struct Config {
   static constexpr int kRowStageBytes = kBBytes + kScaleBytes;
   // Tensor memory columns: accumulators, then each stage's scales.
   static constexpr int kAccColumns = kN < 32 ? 32 : kN;
-  static constexpr int kAccs = kN <= 192 ? 2 : 1;
-  static constexpr int kScaleColumns = 8 * (1 + kBTiles);
+  static constexpr int kAccs = 2;
+  static constexpr int kScaleColumns = 16;
   // Columns that an epilogue warp takes (with 16 rows the second warp of a
   // quarter has none).
   static constexpr int kPart = kN < 32 ? 16 : kN / 2;
@@ -80,6 +79,7 @@ struct Config {
 struct GemmParams {
   CUtensorMap a;  // weights [groups][out][row bytes]
   CUtensorMap b;  // rows [rows][row bytes]
+  CUtensorMap a_scale_map, b_scale_map;  // [tiles][128 words], pairs only
   const uint8_t* a_scales;
   const uint8_t* b_scales;
   const float* bias;
@@ -99,6 +99,7 @@ struct GemmParams {
   int32_t k_tiles;
   int32_t k_stages;
   int32_t m_tiles;
+  int32_t m_pairs;         // of feature tiles
   int32_t activation;
   int32_t paired;          // bf16 y: 4-byte aligned pairs of features
   int32_t split;           // blocks of a cluster that share a tile's k
@@ -248,6 +249,67 @@ __device__ __forceinline__ void WaitLoads() {
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 
+// The forms of a pair of blocks (one on each SM of a pair): issued by its first
+// block for both, arrivals in both.
+__device__ __forceinline__ void CommitPair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster."
+      "multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3))
+      : "memory");
+}
+__device__ __forceinline__ void CopyScalesPair(uint32_t column, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(column),
+               "l"(desc)
+               : "memory");
+}
+__device__ __forceinline__ void MmaPair(uint32_t acc, uint64_t a, uint64_t b,
+                                        uint32_t idesc, uint32_t a_scales,
+                                        uint32_t b_scales, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.u32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X "
+      "[%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(acc),
+      "l"(a), "l"(b), "r"(idesc), "r"(a_scales), "r"(b_scales),
+      "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+// Copies into this block's memory that count at a barrier of either block.
+__device__ __forceinline__ void TmaLoad3Pair(uint32_t dst,
+                                             const CUtensorMap* map, int x,
+                                             int y, int z, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::"
+      "complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void TmaLoad2Pair(uint32_t dst,
+                                             const CUtensorMap* map, int x,
+                                             int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::"
+      "complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ uint32_t AddressAt(uint32_t address, int rank) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(at)
+               : "r"(address), "r"(rank));
+  return at;
+}
+
+// Arrives at the barrier at `bar` of block `rank` of the cluster.
+__device__ __forceinline__ void BarrierArriveAt(uint32_t bar, int rank) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(
+                   AddressAt(bar, rank))
+               : "memory");
+}
+
 __device__ __forceinline__ void ClusterSync() {
   asm volatile(
       "barrier.cluster.arrive.release.aligned;\n\t"
@@ -279,12 +341,12 @@ __device__ __forceinline__ uint64_t ScaleDesc(uint32_t address) {
 
 // Instruction descriptor of kind::mxf4: E2M1 x E2M1, E8M0 scales, K-major
 // operands, dense; `half` selects the scale bytes 0-1 or 2-3 of a column.
-template <int kN>
+template <int kN, int kRowsOfA = kM>
 __device__ __forceinline__ uint32_t InstructionDesc(uint32_t half) {
   const uint32_t id = half * 2;
   return (id << 4) | (1u << 7) | (1u << 10) |
          (static_cast<uint32_t>(kN / 8) << 17) | (1u << 23) |
-         (static_cast<uint32_t>(kM / 16) << 24) | (id << 29);
+         (static_cast<uint32_t>(kRowsOfA / 16) << 24) | (id << 29);
 }
 
 // -------------------------------------------------------------------- tiles
@@ -299,13 +361,12 @@ struct Tile {
 
 // Groups' first row tiles (a running count) and rows in shared memory.
 template <int kN>
-__device__ __forceinline__ Tile TileOf(const GemmParams& p, int item,
-                                       const int* tile_begin,
+__device__ __forceinline__ Tile TileOf(const GemmParams& p, int m_tiles,
+                                       int item, const int* tile_begin,
                                        const int* row_begin) {
-  using C = Config<kN>;
   Tile t;
-  const int n = item / p.m_tiles;
-  t.m = item - n * p.m_tiles;
+  const int n = item / m_tiles;
+  t.m = item - n * m_tiles;
   t.group = 0;
   int64_t at = n;
   int64_t first = 0, count = p.rows;
@@ -327,8 +388,56 @@ __device__ __forceinline__ Tile TileOf(const GemmParams& p, int item,
   t.row = first + at * kN;
   const int64_t left = count - at * kN;
   t.rows = static_cast<int>(left < kN ? left : kN);
-  t.b_tile = (first / kN + t.group + at) * C::kBTiles;
+  // ExpertScaleTiles; with one group a tile of rows' own. A tile of 256 rows
+  // has two scale tiles.
+  t.b_tile = (first / kN + t.group + at) * (kN > kMxTileRows ? 2 : 1);
   return t;
+}
+
+// The plan's offsets, held to [0, rows], and a scan of the row tiles; called by
+// the whole block, which meets once more before it reads them.
+template <int kN>
+__device__ __forceinline__ void ScanOffsets(const GemmParams& p, int warp,
+                                            int lane, int* tile_begin,
+                                            int* row_begin) {
+  if (p.offsets == nullptr) return;
+  if (warp >= 2) {
+    for (int i = threadIdx.x - 64; i <= p.groups; i += blockDim.x - 64) {
+      row_begin[i] =
+          min(max(__ldg(p.offsets + i), 0), static_cast<int>(p.rows));
+    }
+  }
+  __syncthreads();
+  if (warp != 2) return;
+  int carry = 0;
+  for (int base = 0; base <= p.groups; base += 32) {
+    const int i = base + lane;
+    const int count = i < p.groups ? row_begin[i + 1] - row_begin[i] : 0;
+    const int tiles = count > 0 ? (count + kN - 1) / kN : 0;
+    int scan = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += up;
+    }
+    if (i <= p.groups) tile_begin[i] = carry + scan - tiles;
+    carry += __shfl_sync(0xffffffffu, scan, 31);
+  }
+}
+
+// After a failure the copies in flight still have to land: waits (bounded) for
+// the last ones issued before `stage` of `phase`.
+__device__ __forceinline__ void DrainStages(uint64_t* full_bar, int stage,
+                                            uint32_t phase, int64_t issued,
+                                            int stages) {
+  volatile int ignored = 0;
+  for (int64_t i = 0; i < issued && i < stages; ++i) {
+    if (--stage < 0) {
+      stage = stages - 1;
+      phase ^= 1;
+    }
+    if (!BarrierWait(SharedAddress(full_bar + stage), phase, &ignored)) break;
+  }
 }
 
 __device__ __forceinline__ float Activate(float v, int activation) {
@@ -408,6 +517,22 @@ __device__ __forceinline__ void StoreRows(T* y, int64_t stride,
   }
 }
 
+// Zeros in the rows behind the last group's, by the epilogue's warps.
+template <typename T>
+__device__ __forceinline__ void ZeroRowsBehind(const GemmParams& p,
+                                               const int* row_begin) {
+  if (p.offsets == nullptr) return;
+  const int64_t kept = row_begin[p.groups];
+  const int64_t total = (p.rows - kept) * p.out;
+  constexpr int kStep = 32 * kEpilogueWarps;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStep + threadIdx.x - 64;
+       i < total; i += static_cast<int64_t>(gridDim.x) * kStep) {
+    const int64_t r = i / p.out;
+    Store(static_cast<T*>(p.y) + (kept + r) * p.y_stride + (i - r * p.out),
+          0.0f);
+  }
+}
+
 // The 32 elements of a block of x in registers.
 template <typename X>
 struct XBlock {
@@ -469,7 +594,7 @@ __device__ __forceinline__ void QuantizeTiles(
   uint32_t phase = 0;
   for (int item = first_item; item < last_item;
        item = (item / p.m_tiles + 1) * p.m_tiles) {
-    const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+    const Tile t = TileOf<kN>(p, p.m_tiles, item, tile_begin, row_begin);
     const bool ok = BarrierWait(SharedAddress(rows_empty_bar + buffer),
                                 phase ^ 1, failed);
     if (!__all_sync(0xffffffffu, ok)) break;
@@ -570,32 +695,7 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
       asm volatile("prefetch.tensormap [%0];" ::"l"(&p.b) : "memory");
     }
   }
-  if (p.offsets != nullptr) {
-    // The plan's offsets, held to [0, rows], and a scan of the row tiles.
-    if (warp >= 2) {
-      for (int i = threadIdx.x - 64; i <= p.groups; i += blockDim.x - 64) {
-        row_begin[i] = min(max(__ldg(p.offsets + i), 0),
-                           static_cast<int>(p.rows));
-      }
-    }
-    __syncthreads();
-    if (warp == 2) {
-      int carry = 0;
-      for (int base = 0; base <= p.groups; base += 32) {
-        const int i = base + lane;
-        const int count = i < p.groups ? row_begin[i + 1] - row_begin[i] : 0;
-        const int tiles = count > 0 ? (count + kN - 1) / kN : 0;
-        int scan = tiles;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int up = __shfl_up_sync(0xffffffffu, scan, o);
-          if (lane >= o) scan += up;
-        }
-        if (i <= p.groups) tile_begin[i] = carry + scan - tiles;
-        carry += __shfl_sync(0xffffffffu, scan, 31);
-      }
-    }
-  }
+  ScanOffsets<kN>(p, warp, lane, tile_begin, row_begin);
   FenceBeforeSync();
   __syncthreads();
   FenceAfterSync();
@@ -628,14 +728,13 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
     int64_t issued = 0;
     for (int item = first_item; ok && item < last_item;
          item += item_step) {
-      const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+      const Tile t = TileOf<kN>(p, p.m_tiles, item, tile_begin, row_begin);
       const uint8_t* a_scales =
           p.a_scales + (static_cast<int64_t>(t.group) * p.m_tiles + t.m) *
                            p.k_tiles * kMxTileBytes;
       const uint8_t* b_scales =
           p.b_scales + t.b_tile * p.k_tiles * kMxTileBytes;
-      const bool b_first = !kRows && t.b_tile < p.b_tiles;
-      const bool b_second = C::kBTiles == 2 && t.b_tile + 1 < p.b_tiles;
+      const bool b_there = !kRows && t.b_tile < p.b_tiles;
       for (int s = k_begin; s < k_end; ++s) {
         ok = BarrierWait(SharedAddress(empty_bar + stage), phase ^ 1, &failed);
         ok = __all_sync(0xffffffffu, ok);
@@ -647,7 +746,7 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
           const uint32_t bytes =
               2 * s + 1 < p.k_tiles ? kScaleBytes : kMxTileBytes;
           BarrierExpect(bar, kABytes + (kRows ? 0 : C::kBBytes) +
-                                 bytes * (1 + b_first + b_second));
+                                 bytes * (1 + b_there));
           TmaLoad3(at, &p.a, s * (kStageK / 2), t.m * kM, t.group, bar);
           if constexpr (!kRows) {
             TmaLoad2(at + kABytes, &p.b, s * (kStageK / 2),
@@ -655,12 +754,8 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
           }
           const int64_t k_at = static_cast<int64_t>(2 * s) * kMxTileBytes;
           BulkLoad(scales, a_scales + k_at, bytes, bar);
-          if (b_first) {
+          if (b_there) {
             BulkLoad(scales + kScaleBytes, b_scales + k_at, bytes, bar);
-          }
-          if (b_second) {
-            BulkLoad(scales + 2 * kScaleBytes,
-                     b_scales + p.k_tiles * kMxTileBytes + k_at, bytes, bar);
           }
         }
         __syncwarp();
@@ -671,21 +766,7 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
         }
       }
     }
-    // After a failure the copies in flight still have to land.
-    if (!ok) {
-      volatile int ignored = 0;
-      const int in_flight =
-          static_cast<int>(issued < num_stages ? issued : num_stages);
-      for (int i = 0; i < in_flight; ++i) {
-        if (--stage < 0) {
-          stage = num_stages - 1;
-          phase ^= 1;
-        }
-        if (!BarrierWait(SharedAddress(full_bar + stage), phase, &ignored)) {
-          break;
-        }
-      }
-    }
+    if (!ok) DrainStages(full_bar, stage, phase, issued, num_stages);
   } else if (warp == 1) {
     int stage = 0, acc = 0, rows = 0;
     uint32_t phase = 0, acc_phase = 0, rows_phase = 0;
@@ -733,17 +814,13 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
             if (h * 128 >= left) break;
             // Descriptors count 16 bytes.
             CopyScales(a_col + h * 4, a_scales + h * (kMxTileBytes / 16));
-#pragma unroll
-            for (int q = 0; q < C::kBTiles; ++q) {
-              CopyScales(b_col + (h * C::kBTiles + q) * 4,
-                         b_scales + (q * kScaleBytes + h * kMxTileBytes) / 16);
-            }
+            CopyScales(b_col + h * 4, b_scales + h * (kMxTileBytes / 16));
           }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (j * 64 >= left) break;
             Mma(d, a_desc + j * 2, b_desc + j * 2, InstructionDesc<kN>(j & 1),
-                a_col + (j >> 1) * 4, b_col + (j >> 1) * 4 * C::kBTiles,
+                a_col + (j >> 1) * 4, b_col + (j >> 1) * 4,
                 s > k_begin || j > 0);
           }
           Commit(SharedAddress(empty_bar + stage));
@@ -789,7 +866,7 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int item = first_item; item < last_item; item += item_step) {
-      const Tile t = TileOf<kN>(p, item, tile_begin, row_begin);
+      const Tile t = TileOf<kN>(p, p.m_tiles, item, tile_begin, row_begin);
       const int feature = t.m * kM + quarter * 32 + lane;
       const bool mine = feature < p.out;
       const float bias =
@@ -837,19 +914,7 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
         }
       }
     }
-    // Rows behind the last group's.
-    if (p.offsets != nullptr) {
-      const int64_t kept = row_begin[p.groups];
-      const int64_t total = (p.rows - kept) * p.out;
-      const int thread = threadIdx.x - 64;
-      constexpr int kStep = 32 * kEpilogueWarps;
-      for (int64_t i = static_cast<int64_t>(blockIdx.x) * kStep + thread;
-           i < total; i += static_cast<int64_t>(gridDim.x) * kStep) {
-        const int64_t r = i / p.out;
-        Store(static_cast<T*>(p.y) + (kept + r) * p.y_stride + (i - r * p.out),
-              0.0f);
-      }
-    }
+    ZeroRowsBehind<T>(p, row_begin);
   }
   if (p.split > 1) {
     // One tile per cluster; all its blocks come here, also without a tile.
@@ -857,7 +922,7 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
     ClusterSync();
     if (warp >= 2 && warp < 2 + kEpilogueWarps && first_item < last_item &&
         !failed) {
-      const Tile t = TileOf<kN>(p, first_item, tile_begin, row_begin);
+      const Tile t = TileOf<kN>(p, p.m_tiles, first_item, tile_begin, row_begin);
       const int lane_feature = (warp & 3) * 32 + lane;
       const int feature = t.m * kM + lane_feature;
       const float bias =
@@ -888,6 +953,241 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
   }
 }
 
+// ------------------------------------------------------------ pairs of blocks
+
+// Many rows: the blocks of a pair of SMs share tiles of 256 features x 256
+// rows. Each holds the weights of its 128 features and half of the rows, and
+// the pair's MMAs (issued by its first block) read both halves. An SM takes in
+// 64 bytes a cycle from L2 and moves 128 through its shared memory, and both
+// bound the products: the pair's 35 KB a stage need 560 cycles against its
+// MMAs' 512, a block by itself 51 KB for 128 x 256 (8192 x 4096 -> 8192: 114 us,
+// in pairs 104 us). Every block has its own accumulator, scales and epilogue.
+struct Pair {
+  static constexpr int kN = 256;
+  static constexpr int kBBytes = kN / 2 * kStageK / 2;
+  static constexpr int kStageBytes = kABytes + kBBytes + 3 * kScaleBytes;
+  static constexpr int kStages = (217 * 1024) / kStageBytes;
+  // Tensor memory: the accumulator, then the scales of every stage, free once
+  // its last MMAs are done, which the stage's empty barrier has shown.
+  static constexpr int kScaleColumns = 24;
+  static_assert(kN + kStages * kScaleColumns <= 512, "tensor memory");
+  static constexpr int kPart = kN / 2;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    MxPairKernel(const __grid_constant__ GemmParams p) {
+  using C = Pair;
+  constexpr int kN = C::kN;
+  extern __shared__ uint8_t raw[];
+  __shared__ alignas(8) uint64_t full_bar[C::kStages];
+  __shared__ alignas(8) uint64_t empty_bar[C::kStages];
+  __shared__ alignas(8) uint64_t acc_full_bar;
+  __shared__ alignas(8) uint64_t acc_empty_bar;
+  __shared__ uint32_t tmem_base;
+  __shared__ volatile int failed;
+
+  uint8_t* stages = raw + (1024 - (SharedAddress(raw) & 1023)) % 1024;
+  int* tile_begin =
+      reinterpret_cast<int*>(stages + C::kStages * C::kStageBytes);
+  int* row_begin = tile_begin + (p.groups + 1);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x / 32, 0);
+  const int lane = threadIdx.x & 31;
+  const int rank = blockIdx.x & 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      BarrierInit(SharedAddress(full_bar + i), 1);
+      BarrierInit(SharedAddress(empty_bar + i), 1);
+    }
+    BarrierInit(SharedAddress(&acc_full_bar), 1);
+    BarrierInit(SharedAddress(&acc_empty_bar), 2 * kEpilogueWarps);
+    failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == 0 && Elect()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.a) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.b) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.a_scale_map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&p.b_scale_map) : "memory");
+  }
+  ScanOffsets<kN>(p, warp, lane, tile_begin, row_begin);
+  // Both blocks' barriers are there before either's copies, and both blocks
+  // before the pair's allocation.
+  __syncwarp();
+  ClusterSync();
+  if (warp == 1) {
+    asm volatile(
+        "tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;"
+        ::"r"(SharedAddress(&tmem_base))
+        : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;"
+                 ::: "memory");
+  }
+  FenceBeforeSync();
+  __syncthreads();
+  FenceAfterSync();
+  __syncwarp();
+  ClusterSync();  // both blocks' tensor memory is there
+  const uint32_t tmem = tmem_base;
+  const int row_tiles = p.offsets != nullptr
+                            ? tile_begin[p.groups]
+                            : static_cast<int>((p.rows + kN - 1) / kN);
+  const int items = row_tiles * p.m_pairs;
+  const int first_item = blockIdx.x / 2, item_step = gridDim.x / 2;
+  const uint32_t stage_base = SharedAddress(stages);
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    int64_t issued = 0;
+    for (int item = first_item; ok && item < items; item += item_step) {
+      const Tile t = TileOf<kN>(p, p.m_pairs, item, tile_begin, row_begin);
+      // A pair's second block may lie behind the last features (its codes then
+      // read as zeros, its scales are some other tile's), and a tile's second
+      // scales behind the last ones: no result depends on them.
+      const int m = t.m * 2 + rank;
+      const int a_tile = (t.group * p.m_tiles + m) * p.k_tiles;
+      const int b_tile = static_cast<int>(t.b_tile) * p.k_tiles;
+      for (int s = 0; s < p.k_stages; ++s) {
+        ok = BarrierWait(SharedAddress(empty_bar + stage), phase ^ 1, &failed);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (Elect()) {
+          // All copies of both blocks count at the first block's barrier.
+          const uint32_t bar = AddressAt(SharedAddress(full_bar + stage), 0);
+          const uint32_t at = stage_base + stage * C::kStageBytes;
+          const uint32_t scales = at + kABytes + C::kBBytes;
+          if (rank == 0) {
+            BarrierExpect(SharedAddress(full_bar + stage),
+                          2 * C::kStageBytes);
+          }
+          TmaLoad3Pair(at, &p.a, s * (kStageK / 2), m * kM, t.group, bar);
+          TmaLoad2Pair(at + kABytes, &p.b, s * (kStageK / 2),
+                       static_cast<int>(t.row) + rank * (kN / 2), bar);
+          TmaLoad2Pair(scales, &p.a_scale_map, 0, a_tile + 2 * s, bar);
+          TmaLoad2Pair(scales + kScaleBytes, &p.b_scale_map, 0, b_tile + 2 * s,
+                       bar);
+          TmaLoad2Pair(scales + 2 * kScaleBytes, &p.b_scale_map, 0,
+                       b_tile + p.k_tiles + 2 * s, bar);
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok && rank == 0) {
+      DrainStages(full_bar, stage, phase, issued, C::kStages);
+    }
+  } else if (warp == 1 && rank == 0) {
+    int stage = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true;
+    for (int item = first_item; ok && item < items; item += item_step) {
+      ok = BarrierWait(SharedAddress(&acc_empty_bar), acc_phase ^ 1, &failed);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      for (int s = 0; s < p.k_stages; ++s) {
+        ok = BarrierWait(SharedAddress(full_bar + stage), phase, &failed);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        FenceAfterSync();
+        if (Elect()) {
+          const uint32_t at = stage_base + stage * C::kStageBytes;
+          const uint32_t a_col = tmem + kN + stage * C::kScaleColumns;
+          const uint32_t b_col = a_col + 8;
+          const uint64_t a_desc = SwizzledDesc(at);
+          const uint64_t b_desc = SwizzledDesc(at + kABytes);
+          const uint64_t scales = ScaleDesc(at + kABytes + C::kBBytes);
+          const int left = p.k - s * kStageK;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h * 128 >= left) break;
+            const uint64_t half = scales + h * (kMxTileBytes / 16);
+            CopyScalesPair(a_col + h * 4, half);
+            CopyScalesPair(b_col + h * 8, half + kScaleBytes / 16);
+            CopyScalesPair(b_col + h * 8 + 4, half + 2 * kScaleBytes / 16);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (j * 64 >= left) break;
+            MmaPair(tmem, a_desc + j * 2, b_desc + j * 2,
+                    InstructionDesc<kN, 2 * kM>(j & 1), a_col + (j >> 1) * 4,
+                    b_col + (j >> 1) * 8, s > 0 || j > 0);
+          }
+          CommitPair(SharedAddress(empty_bar + stage));
+        }
+        __syncwarp();
+        if (++stage == C::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (!ok) break;
+      if (Elect()) CommitPair(SharedAddress(&acc_full_bar));
+      __syncwarp();
+      acc_phase ^= 1;
+    }
+  } else if (warp >= 2) {
+    const int quarter = warp & 3;
+    const int first_column = (warp - 2) / 4 * C::kPart;
+    uint32_t acc_phase = 0;
+    for (int item = first_item; item < items; item += item_step) {
+      const Tile t = TileOf<kN>(p, p.m_pairs, item, tile_begin, row_begin);
+      const int feature = (t.m * 2 + rank) * kM + quarter * 32 + lane;
+      const bool mine = feature < p.out;
+      const float bias =
+          p.bias != nullptr && mine
+              ? __ldg(p.bias + static_cast<int64_t>(t.group) * p.out + feature)
+              : 0.0f;
+      const bool ok =
+          BarrierWait(SharedAddress(&acc_full_bar), acc_phase, &failed);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      FenceAfterSync();
+      const uint32_t d = tmem + first_column +
+                         (static_cast<uint32_t>(quarter * 32) << 16);
+      const bool some = first_column < t.rows;
+      uint32_t r[C::kPart];
+      if (some) {
+#pragma unroll
+        for (int c = 0; c < C::kPart; c += 16) LoadColumns(d + c, r + c);
+        WaitLoads();
+      }
+      FenceBeforeSync();
+      __syncwarp();
+      if (lane == 0) BarrierArriveAt(SharedAddress(&acc_empty_bar), 0);
+      acc_phase ^= 1;
+      if (!some) continue;
+      T* y = static_cast<T*>(p.y) + (t.row + first_column) * p.y_stride +
+             feature;
+      const int rows = t.rows - first_column;
+#pragma unroll
+      for (int c = 0; c < C::kPart; c += 16) {
+        if (c >= rows) break;
+        StoreRows(y + c * p.y_stride, p.y_stride, r + c, bias, p.activation,
+                  rows - c, mine, p.paired, lane);
+      }
+    }
+    ZeroRowsBehind<T>(p, row_begin);
+  }
+  // Neither block ends while the other may still arrive at its barriers or
+  // read its stages.
+  __syncwarp();
+  FenceBeforeSync();
+  ClusterSync();
+  if (warp == 1) {
+    FenceAfterSync();
+    asm volatile(
+        "tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem)
+        : "memory");
+  }
+}
+
 // ------------------------------------------------------------------- launch
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t,
@@ -913,14 +1213,29 @@ EncodeTiled GetEncodeTiled() {
   return fn;
 }
 
-// [groups][rows][row bytes] of codes as boxes of 128 bytes x `box_rows`,
-// swizzled; parts of a box outside the matrix read as zero codes.
-int EncodeCodes(CUtensorMap* map, const void* codes, int64_t row_bytes,
-                int64_t rows, int64_t groups, int rank, int box_rows) {
+int Encode(CUtensorMap* map, CUtensorMapDataType type, const void* base,
+           int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+           const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
   EncodeTiled encode = GetEncodeTiled();
   if (encode == nullptr) {
     return FailWith(XSE_INTERNAL, "cuTensorMapEncodeTiled is not available");
   }
+  const cuuint32_t steps[3] = {1, 1, 1};
+  const CUresult r = encode(map, type, rank, const_cast<void*>(base), dims,
+                            strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return FailWith(XSE_INTERNAL, "tensor map of a 4-bit matrix: error %d",
+                    static_cast<int>(r));
+  }
+  return XSE_OK;
+}
+
+// [groups][rows][row bytes] of codes as boxes of 128 bytes x `box_rows`,
+// swizzled; parts of a box outside the matrix read as zero codes.
+int EncodeCodes(CUtensorMap* map, const void* codes, int64_t row_bytes,
+                int64_t rows, int64_t groups, int rank, int box_rows) {
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(row_bytes),
                               static_cast<cuuint64_t>(rows),
                               static_cast<cuuint64_t>(groups)};
@@ -928,17 +1243,18 @@ int EncodeCodes(CUtensorMap* map, const void* codes, int64_t row_bytes,
                                  static_cast<cuuint64_t>(row_bytes * rows)};
   const cuuint32_t box[3] = {kStageK / 2, static_cast<cuuint32_t>(box_rows),
                              1};
-  const cuuint32_t steps[3] = {1, 1, 1};
-  const CUresult r = encode(
-      map, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(codes), dims,
-      strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) {
-    return FailWith(XSE_INTERNAL, "tensor map of 4-bit codes: error %d",
-                    static_cast<int>(r));
-  }
-  return XSE_OK;
+  return Encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, codes, rank, dims, strides,
+                box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Scale tiles as rows of 128 words, in boxes of a stage's two.
+int EncodeScales(CUtensorMap* map, const void* scales, int64_t tiles) {
+  const cuuint64_t dims[2] = {kMxTileBytes / 4,
+                              static_cast<cuuint64_t>(tiles)};
+  const cuuint64_t strides[1] = {kMxTileBytes};
+  const cuuint32_t box[2] = {kMxTileBytes / 4, 2};
+  return Encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, scales, 2, dims, strides,
+                box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 template <int kN, typename T, typename X>
@@ -981,6 +1297,53 @@ int LaunchGemmAs(GemmParams& p, const void* a_codes, const void* b_codes,
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, MxGemmKernel<kN, T, X>, p);
+  }
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return FailWith(XSE_INTERNAL, "4-bit product launch: %s",
+                    cudaGetErrorString(e));
+  }
+  return XSE_OK;
+}
+
+// Many rows, by pairs of blocks.
+template <typename T>
+int LaunchPairAs(GemmParams& p, const void* a_codes, const void* b_codes,
+                 int64_t row_tiles, cudaStream_t s) {
+  const int64_t row_bytes = MxRowBytes(p.k);
+  int rc = EncodeCodes(&p.a, a_codes, row_bytes, p.out, p.groups, 3, kM);
+  if (rc == XSE_OK) {
+    rc = EncodeCodes(&p.b, b_codes, row_bytes, p.rows, 1, 2, Pair::kN / 2);
+  }
+  if (rc == XSE_OK) {
+    rc = EncodeScales(&p.a_scale_map, p.a_scales,
+                      static_cast<int64_t>(p.groups) * p.m_tiles * p.k_tiles);
+  }
+  if (rc == XSE_OK) {
+    rc = EncodeScales(&p.b_scale_map, p.b_scales, p.b_tiles * p.k_tiles);
+  }
+  if (rc != XSE_OK) return rc;
+  p.m_pairs = (p.m_tiles + 1) / 2;
+  constexpr size_t kFixed = 1024 + Pair::kStages * Pair::kStageBytes;
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = AllowShared(MxPairKernel<T>,
+                              kFixed + 8 * (XSE_MAX_EXPERTS + 1), &allowed);
+  if (e == cudaSuccess) {
+    const int64_t pairs = row_tiles * p.m_pairs;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(
+        2 * (pairs > kNumSms / 2 ? kNumSms / 2 : pairs)));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes =
+        kFixed + (p.offsets != nullptr ? 8 * (p.groups + 1) : 0);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, MxPairKernel<T>, p);
   }
   if (e != cudaSuccess) {
     cudaGetLastError();
@@ -1085,10 +1448,11 @@ int RunGemm(const Rows& from, int64_t rows, const xse_mx_matrix& w,
       return LaunchGemm<64>(p, y_dtype, w.codes, from.codes, items, s);
     case 128:
       return LaunchGemm<128>(p, y_dtype, w.codes, from.codes, items, s);
-    case 192:
-      return LaunchGemm<192>(p, y_dtype, w.codes, from.codes, items, s);
     default:
-      return LaunchGemm<256>(p, y_dtype, w.codes, from.codes, items, s);
+      return y_dtype == XSE_DT_BF16
+                 ? LaunchPairAs<__nv_bfloat16>(p, w.codes, from.codes,
+                                               row_tiles, s)
+                 : LaunchPairAs<float>(p, w.codes, from.codes, row_tiles, s);
   }
 }
 
@@ -1195,8 +1559,7 @@ int xse_linear_forward_mxfp4_q(const xse_mx_matrix* x, const xse_mx_matrix* w,
     return FailWith(XSE_INVALID_ARGUMENT,
                     "4-bit layer buffers must be non-null.");
   }
-  // Scale tiles of 128 rows serve tiles of 256.
-  const int n = x->rows > 128 ? 256 : MxTileRowsFor(x->rows, 1, w->cols);
+  const int n = MxTileRowsFor(x->rows, 1, w->cols);
   Rows from{};
   from.codes = x->codes;
   from.scales = x->scales;
@@ -1212,8 +1575,7 @@ int64_t xse_linear_mxfp4_workspace(int64_t rows, int32_t in_dim) {
   const int n = xse::MxTileRowsFor(rows, 1, in_dim);
   if (xse::MxQuantizesInProduct(n, in_dim)) return 0;
   return rows * xse::MxRowBytes(in_dim) +
-         xse::MxProductTiles(rows, n) * xse::MxKTiles(in_dim) *
-             xse::kMxTileBytes;
+         xse::MxRowTiles(rows) * xse::MxKTiles(in_dim) * xse::kMxTileBytes;
 }
 
 int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
@@ -1244,7 +1606,7 @@ int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
   }
   const int n = MxTileRowsFor(rows, 1, w->cols);
   return RunLayer(x, x_dtype, rows, x_stride, rows, false, nullptr,
-                  MxProductTiles(rows, n), *w, bias, activation, n, y, y_dtype,
+                  MxRowTiles(rows), *w, bias, activation, n, y, y_dtype,
                   y_stride, workspace, static_cast<cudaStream_t>(stream));
 }
 

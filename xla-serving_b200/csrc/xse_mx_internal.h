@@ -61,21 +61,14 @@ int CheckExpertPlan(const xse_expert_plan* plan);
 // Rows of a product's tile for groups of rows / groups rows on average. The
 // scales of an expert product's rows are laid out in 512-byte tiles of that
 // many rows each, so that every tile's scales begin a column of tensor memory.
-// 256 rows read the least shared memory per product but leave no room for a
-// second accumulator, which a long k makes up for: 8192 rows to 8192 features,
-// 192 and 256 rows a tile: k 2048 84.6 and 99.5 us, k 4096 143 and 134 us. 128
-// rows: 103 and 180 us.
+// 256 rows (pairs of SMs) need a k that is long against the end of a tile,
+// which nothing overlaps there: 8192 rows to 8192 features in bf16, tiles of 128
+// and 256 rows, quantisation included: k 1024 60 and 68 us, k 2048 85 and 75 us,
+// k 4096 146 and 121 us; 64 experts' 512 rows each, k 2048: 111 and 106 us.
 inline int MxTileRowsFor(int64_t rows, int32_t groups, int32_t k) {
   const int64_t mean = (rows + groups - 1) / groups;
   if (mean <= 64) return mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
-  if (mean <= 128) return 128;
-  return groups == 1 && k >= 4096 ? 256 : 192;
-}
-
-// Scale tiles of n-row tiles over `rows` rows of one group: a tile of more
-// than 128 rows has two.
-inline int64_t MxProductTiles(int64_t rows, int n) {
-  return (rows + n - 1) / n * (n > kMxTileRows ? 2 : 1);
+  return mean <= 128 || k < 1536 ? 128 : 256;
 }
 
 // Scale tiles of n rows that hold every expert's rows on tile boundaries:
@@ -99,9 +92,9 @@ inline bool MxQuantizesInProduct(int n, int32_t k) {
 }
 
 // Quantises the rows of x for a product in tiles of `tile_rows`: plan NULL, one
-// group whose scales lie as MxProductTiles says (as xse_mxfp4_quantize lays
-// them out where tile_rows <= 128); else to the sorted rows' places (codes by sorted
-// row, scales as ExpertScaleTiles says), from token rows or sorted ones.
+// group as xse_mxfp4_quantize lays it out; else to the sorted rows' places
+// (codes by sorted row, scales as ExpertScaleTiles says), from token rows or
+// sorted ones.
 int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
                  int64_t row_stride, const xse_expert_plan* plan, bool sorted,
                  int tile_rows, void* codes, void* scales,
