@@ -106,7 +106,7 @@ struct QuantParams {
   int32_t k_tiles;
   int64_t row_bytes;
   int64_t row_tiles;    // scale tiles of a group's rows (of all: with a plan)
-  int32_t tile_rows;    // rows of a product's tile
+  int32_t tile_shift;   // of a product's tile: 2^tile_shift rows
   uint8_t* codes;
   uint8_t* scales;
   const int32_t* offsets;
@@ -154,32 +154,69 @@ __device__ __forceinline__ const T* RowOf(const QuantParams& p, int64_t row) {
          (row - g * p.rows) * p.row_stride;
 }
 
-// Calls put(code row, scale row) for each place of source row `row`.
+// Where a source row's quantised row goes: its code row, -1 for nowhere, and its
+// row of scales.
+struct Place {
+  int32_t code_row;
+  int64_t scale_row;
+};
+
+// The places of choices [first, first + 32) of a row, lane by lane.
+template <int kMode>
+__device__ __forceinline__ Place PlaceOf(const QuantParams& p, int64_t row,
+                                         int choice) {
+  Place none{-1, 0};
+  int32_t slot = static_cast<int32_t>(row);
+  if (kMode == kFromTokens) {
+    if (choice >= p.topk) return none;
+    slot = __ldg(p.slots + row * p.topk + choice);
+  }
+  if (slot < 0 || slot >= p.pairs) return none;
+  // The experts that end at or before the row.
+  int low = 0, high = p.num_experts;
+  while (low < high) {
+    const int mid = (low + high) / 2;
+    if (__ldg(p.offsets + mid + 1) <= slot) {
+      low = mid + 1;
+    } else {
+      high = mid;
+    }
+  }
+  if (low == p.num_experts) return none;  // behind the last sorted row
+  const int32_t begin = __ldg(p.offsets + low);
+  if (begin < 0 || begin > slot) return none;
+  // Tiles have 2^tile_shift rows, those of 256 two scale tiles.
+  const int local = slot - begin;
+  const int in_tile = local & ((1 << p.tile_shift) - 1);
+  const int64_t tile =
+      (static_cast<int64_t>(begin >> p.tile_shift) + low +
+       (local >> p.tile_shift)) *
+          (1 << p.tile_shift > kMxTileRows ? 2 : 1) +
+      in_tile / kMxTileRows;
+  if (tile >= p.row_tiles) return none;
+  return Place{slot, tile * kMxTileRows + in_tile % kMxTileRows};
+}
+
+// Calls put(code row, scale row) for each place of source row `row`; all lanes
+// of the warp together.
 template <int kMode, typename Put>
 __device__ __forceinline__ void ForPlaces(const QuantParams& p, int64_t row,
                                           int lane, Put put) {
   if constexpr (kMode == kPlain) {
     const int64_t g = p.groups == 1 ? 0 : row / p.rows;
     put(row, g * p.row_tiles * kMxTileRows + (row - g * p.rows));
+  } else if constexpr (kMode == kFromSorted) {
+    const Place at = PlaceOf<kMode>(p, row, 0);
+    if (at.code_row >= 0) put(at.code_row, at.scale_row);
   } else {
-    const int count = kMode == kFromTokens ? p.topk : 1;
-    for (int j = 0; j < count; ++j) {
-      const int32_t slot = kMode == kFromTokens
-                               ? __ldg(p.slots + row * p.topk + j)
-                               : static_cast<int32_t>(row);
-      if (slot < 0 || slot >= p.pairs) continue;
-      const int e = ExpertOfRow(p.offsets, p.num_experts, slot, lane);
-      if (e >= p.num_experts) continue;  // behind the last sorted row
-      const int32_t begin = __ldg(p.offsets + e);
-      if (begin < 0 || begin > slot) continue;
-      const int local = slot - begin;
-      const int in_tile = local % p.tile_rows;
-      const int64_t tile =
-          static_cast<int64_t>(begin / p.tile_rows + e + local / p.tile_rows) *
-              (p.tile_rows > kMxTileRows ? 2 : 1) + in_tile / kMxTileRows;
-      if (tile >= p.row_tiles) continue;
-      put(static_cast<int64_t>(slot),
-          tile * kMxTileRows + in_tile % kMxTileRows);
+    for (int first = 0; first < p.topk; first += 32) {
+      const Place mine = PlaceOf<kMode>(p, row, first + lane);
+      const int count = min(p.topk - first, 32);
+      for (int j = 0; j < count; ++j) {
+        const int64_t code_row = __shfl_sync(0xffffffffu, mine.code_row, j);
+        const int64_t scale_row = __shfl_sync(0xffffffffu, mine.scale_row, j);
+        if (code_row >= 0) put(code_row, scale_row);
+      }
     }
   }
 }
@@ -517,7 +554,7 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
   p.scales = static_cast<uint8_t*>(scales);
   if (plan == nullptr) return RunQuantize(p, dtype, kPlain, stream);
   p.pairs = plan->tokens * plan->topk;
-  p.tile_rows = tile_rows;
+  while ((1 << p.tile_shift) < tile_rows) ++p.tile_shift;
   p.row_tiles = ExpertScaleTiles(p.pairs, plan->num_experts, tile_rows);
   p.offsets = plan->offsets;
   p.slots = plan->slots;

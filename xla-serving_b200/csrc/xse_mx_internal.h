@@ -184,22 +184,6 @@ __device__ __forceinline__ int64_t MxScaleAt(int64_t r, int64_t b,
          ((r >> 5) & 3) * 4 + (b & 3);
 }
 
-// The expert of a sorted row: the number of experts that end at or before it.
-// All lanes of a warp call it together with the same row.
-__device__ __forceinline__ int ExpertOfRow(const int32_t* offsets,
-                                           int num_experts, int row,
-                                           int lane) {
-  int e = 0;
-  for (int base = 0; base < num_experts; base += 32) {
-    const int i = base + lane;
-    const bool before = i < num_experts && __ldg(offsets + i + 1) <= row;
-    const unsigned ballot = __ballot_sync(0xffffffffu, before);
-    e += __popc(ballot);
-    if (ballot != 0xffffffffu) break;
-  }
-  return e;
-}
-
 #endif  // __CUDACC__
 
 }  // namespace xse
