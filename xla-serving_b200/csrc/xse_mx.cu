@@ -237,6 +237,8 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int kSpan = 32 * P::kElements;
   __shared__ uint4 turn[kAligned ? 1 : kThreads / 32]
                        [kAligned ? 1 : 32 * P::kPieces];
+  // A product of these rows may be launched; it waits for this kernel's end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31;
   const int padded = p.k_tiles * 128, code_cols = (p.cols + 31) / 32 * 32;
   const WarpRow w = FirstRow(p.row_shift);
