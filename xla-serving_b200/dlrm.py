@@ -11,7 +11,9 @@ of the reference's DCN-v2 cross network, and the Dense layers with fused
 bias+ReLU (xse_linear_forward): fp32 GEMMs, or -- MATH_TF32X3, what the
 benchmark runs -- three TF32 tensor-core GEMMs over hi/lo split operands
 (fp32-level accuracy). With the fused interaction the interaction kernel
-writes the first top layer's split operands itself.
+writes the first top layer's split operands itself. MATH_MXFP4 runs the layers
+as microscaled 4-bit products (mx.py): activations and kernels in 4 bits, for
+models that were trained or calibrated for it.
 
 Initialisation: Dense kernels Xavier-uniform, biases U(-1/sqrt(fan_in),
 1/sqrt(fan_in)) as the reference's uniform_init (model_jce.py:107-118),
@@ -25,14 +27,17 @@ import numpy as np
 import torch
 
 from . import _capi as C
+from . import mx
 from .engine import BagRequest, EmbeddingEngine, Status, stream_handle
 
 BOTTOM_MLP = (512, 256, 128)
 TOP_MLP = (1024, 1024, 512, 256, 1)
 # Dense-layer arithmetic of the tower: C.MATH_FP32 (CUDA-core fp32 GEMMs),
-# C.MATH_TF32 (one TF32 GEMM: reduced precision), or MATH_TF32X3 (three TF32
-# tensor-core GEMMs over hi/lo split operands: fp32-level accuracy).
+# C.MATH_TF32 (one TF32 GEMM: reduced precision), MATH_TF32X3 (three TF32
+# tensor-core GEMMs over hi/lo split operands: fp32-level accuracy), or
+# MATH_MXFP4 (activations and kernels in microscaled 4 bits, fp32 sums).
 MATH_TF32X3 = 3
+MATH_MXFP4 = 4
 
 
 def interaction_width(num_tables, dim):
@@ -134,6 +139,12 @@ class DenseTower:
           hi, lo = torch.empty_like(k), torch.empty_like(k)
           tf32_split(k, hi, lo)
           self._split[id(layer)] = (hi, lo)
+    # 4-bit layers: all but the 1-wide sigmoid head.
+    self._mx = {}
+    if math == MATH_MXFP4:
+      for layer in self.bottom + self.top:
+        if layer.activation != C.ACT_SIGMOID:
+          self._mx[id(layer)] = mx.quantize(layer.kernel.t())
     self.device = device
     self.math = math
     self._buffers = {}
@@ -235,11 +246,15 @@ class DenseTower:
     return x.view(-1)
 
   def _layer(self, x, layer, out, bufs, stream):
+    weights = self._mx.get(id(layer))
+    if weights is not None:
+      return mx.linear(x[:, :weights.cols], weights, layer.bias,
+                       layer.activation, out, stream=stream)
     split = self._split.get(id(layer))
     if split is not None and x.stride(0) != layer.kernel.shape[0]:
       split = None  # the split buffers are dense [rows, in]
     if split is None:
-      math = C.MATH_FP32 if self.math == MATH_TF32X3 else self.math
+      math = C.MATH_FP32 if self.math >= MATH_TF32X3 else self.math
       return linear(x, layer, out, math=math, stream=stream)
     rows, width = x.shape[0], layer.kernel.shape[0]
     hi = bufs["hi"][:rows * width].view(rows, width)
