@@ -28,8 +28,8 @@
 extern "C" {
 #endif
 
-/* `groups` matrices of [rows, cols] in 4 bits, as one allocation each of
- * codes and scales:
+/* `groups` matrices of [rows, cols] in 4 bits (rows < 2^31, cols <= 2^30), as
+ * one allocation each of codes and scales:
  *   codes: [groups][rows][16 * ceil(cols / 32)] bytes, element 2i in the low
  *          half of byte i; 16-byte aligned
  *   scales: [groups][ceil(rows / 128)][ceil(cols / 128)][512] bytes; block b
@@ -88,7 +88,8 @@ int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
 
 /* Waits for `stream` and reports whether a product's kernel on the current
  * device gave up one of its bounded waits since the last check
- * (DEADLINE_EXCEEDED; its outputs are then incomplete). */
+ * (DEADLINE_EXCEEDED; its outputs are then incomplete). Not for use while a
+ * stream is being captured. */
 int xse_mxfp4_check(void* stream);
 
 #ifdef __cplusplus

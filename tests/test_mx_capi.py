@@ -41,7 +41,8 @@ def test_buffer_sizes(capi):
         groups * tiles * 512
     need = lib.xse_linear_mxfp4_workspace(rows, cols)
     assert need == 0 if rows <= 32 else need >= rows * blocks * 16 + tiles * 512
-  for rows, cols, groups in ((-1, 4, 1), (1, 0, 1), (1, 4, 0), (2 ** 31, 4, 1)):
+  for rows, cols, groups in ((-1, 4, 1), (1, 0, 1), (1, 4, 0), (2 ** 31, 4, 1),
+                             (1, 2 ** 30 + 1, 1)):
     assert lib.xse_mxfp4_codes_bytes(rows, cols, groups) == 0
     assert lib.xse_mxfp4_scales_bytes(rows, cols, groups) == 0
   assert lib.xse_expert_linear_workspace(8, 0, 64) == 0
@@ -90,6 +91,7 @@ def test_matrix_refusals(capi):
   refused(capi, q(matrix(capi, rows=-1)), "rows")
   refused(capi, q(matrix(capi, rows=2 ** 31)), "rows")
   refused(capi, q(matrix(capi, cols=0)), "cols")
+  refused(capi, q(matrix(capi, cols=2 ** 30 + 1)), "cols")
   refused(capi, q(matrix(capi, groups=0)), "groups")
   refused(capi, q(matrix(capi, codes=None)), "non-null")
   refused(capi, q(matrix(capi, codes=4104)), "aligned")
@@ -169,6 +171,8 @@ def test_expert_refusals(capi):
   for call, first in ((gather, "x"), (combine, "y")):
     refused(capi, call(dtype=2), "type 2")
     refused(capi, call(cols=0), "cols")
+    refused(capi, call(cols=2 ** 30 + 1, os=2 ** 31, **{first + "s": 2 ** 31}),
+            "cols")
     refused(capi, call(os=63), "strides")
     refused(capi, call(**{first + "s": 63}), "strides")
     refused(capi, call(**{first: None}), "non-null")

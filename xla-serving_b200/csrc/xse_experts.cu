@@ -1011,8 +1011,9 @@ int CheckRows(const xse_expert_plan* plan, int32_t dtype, int32_t cols) {
     return FailWith(XSE_INVALID_ARGUMENT,
                     "Expert rows are float32 or bfloat16, got type %d", dtype);
   }
-  if (cols < 1) {
-    return FailWith(XSE_INVALID_ARGUMENT, "Expert rows need cols >= 1.");
+  if (cols < 1 || cols > kMostColumns) {
+    return FailWith(XSE_INVALID_ARGUMENT,
+                    "Expert rows need 1 <= cols <= 2^30.");
   }
   return XSE_OK;
 }

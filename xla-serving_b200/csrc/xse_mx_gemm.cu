@@ -1580,7 +1580,10 @@ int xse_linear_forward_mxfp4_q(const xse_mx_matrix* x, const xse_mx_matrix* w,
 }
 
 int64_t xse_linear_mxfp4_workspace(int64_t rows, int32_t in_dim) {
-  if (rows < 1 || rows > INT32_MAX || in_dim < 1) return 0;
+  if (rows < 1 || rows > INT32_MAX || in_dim < 1 ||
+      in_dim > xse::kMostColumns) {
+    return 0;
+  }
   const int n = xse::MxTileRowsFor(rows, 1, in_dim);
   if (xse::MxQuantizesInProduct(n, in_dim)) return 0;
   return rows * xse::MxRowBytes(in_dim) +
@@ -1622,7 +1625,8 @@ int xse_linear_forward_mxfp4(const void* x, int32_t x_dtype, int64_t rows,
 int64_t xse_expert_linear_workspace(int64_t pairs, int32_t num_experts,
                                     int32_t in_dim) {
   if (pairs < 0 || pairs > INT32_MAX || num_experts < 1 ||
-      num_experts > XSE_MAX_EXPERTS || in_dim < 1) {
+      num_experts > XSE_MAX_EXPERTS || in_dim < 1 ||
+      in_dim > xse::kMostColumns) {
     return 0;
   }
   const int n = xse::MxTileRowsFor(pairs, num_experts, in_dim);

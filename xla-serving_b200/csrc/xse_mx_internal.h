@@ -20,6 +20,7 @@ constexpr int kMxBlock = 32;       // elements per scale
 constexpr int kMxTileRows = 128;   // rows of a scale tile
 constexpr int kMxTileBytes = 512;  // 128 rows x 4 blocks
 constexpr int kNumSms = 148;
+constexpr int32_t kMostColumns = 1 << 30;  // of a row: offsets into it fit int
 
 // Sets the error text (printf style) and returns `code`.
 int FailWith(int code, const char* fmt, ...)

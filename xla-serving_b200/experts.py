@@ -19,7 +19,7 @@ import torch
 
 from . import _capi as C
 from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_stream, elsewhere,
-                 float_code, invalid, layer_output, on, row_stride)
+                 invalid, layer_output, matrix, on)
 
 MAX_EXPERTS = 1024
 _INDEX = {torch.int32: C.INDEX_I32, torch.int64: C.INDEX_I64}
@@ -134,14 +134,6 @@ def sort(ids, num_experts, plan=None, *, stream=None) -> ExpertPlan:
   return plan
 
 
-def _rows(t, rows, what):
-  """(columns, row stride) of a tensor with `rows` rows."""
-  stride = row_stride(t, what)
-  if t.shape[0] != rows:
-    raise invalid(f"{what} must have {rows} rows, got shape {tuple(t.shape)}")
-  return t.shape[1], stride
-
-
 def _weights(weights, plan):
   if weights is None:
     return None
@@ -157,22 +149,21 @@ def _weights(weights, plan):
 def _output(out, rows, cols, like, what="out"):
   """(tensor, row stride) of an output of `like`'s type."""
   if out is None:
-    return like.new_empty((rows, cols)), cols
+    return like.new_empty(rows, cols), cols
   if out.shape != (rows, cols) or out.dtype != like.dtype:
     raise invalid(f"{what} must be {like.dtype} of shape {(rows, cols)}, got "
                   f"{out.dtype} {tuple(out.shape)}")
-  return out, row_stride(out, what)
+  return out, matrix(out, what)[3]
 
 
 def gather(x, plan: ExpertPlan, out=None, *, stream=None):
   """x's rows in sorted order: out[r] = x[plan.order[r] // topk], zeros behind
   the last sorted row. Its gradient is combine(grad, plan)."""
-  code = float_code(x, "x")
   index = x.get_device()
   if elsewhere(index, stream):
     with on(index, stream):
       return gather(x, plan, out)
-  cols, stride = _rows(x, plan.tokens, "x")
+  code, _, cols, stride = matrix(x, "x", plan.tokens)
   out, out_stride = _output(out, plan.pairs, cols, x)
   C.check(C.lib.xse_expert_gather(
       x.data_ptr(), code, cols, stride, plan.ref, out.data_ptr(), out_stride,
@@ -184,12 +175,11 @@ def combine(y, plan: ExpertPlan, weights=None, out=None, *, stream=None):
   """out[t] = sum over j of weights[t, j] * y[plan.slots[t, j]] (weights 1
   without them), summed in fp32 in the order of the choices; a row all of
   whose pairs were dropped is zero."""
-  code = float_code(y, "y")
   index = y.get_device()
   if elsewhere(index, stream):
     with on(index, stream):
       return combine(y, plan, weights, out)
-  cols, stride = _rows(y, plan.pairs, "y")
+  code, _, cols, stride = matrix(y, "y", plan.pairs)
   w = _weights(weights, plan)
   out, out_stride = _output(out, plan.tokens, cols, y)
   C.check(C.lib.xse_expert_combine(
@@ -204,19 +194,18 @@ def combine_backward(grad, y, plan: ExpertPlan, weights=None, grad_y=None,
   of pair p gets weights[p] * grad[p // topk] (zeros behind the last), weight
   (t, j) the dot product of grad[t] and its sorted row (0 for a dropped
   pair)."""
-  code = float_code(y, "y")
   index = y.get_device()
   if elsewhere(index, stream):
     with on(index, stream):
       return combine_backward(grad, y, plan, weights, grad_y, grad_weights)
-  cols, y_stride = _rows(y, plan.pairs, "y")
-  grad_cols, grad_stride = _rows(grad, plan.tokens, "grad")
-  if grad.dtype != y.dtype or grad_cols != cols:
+  code, _, cols, y_stride = matrix(y, "y", plan.pairs)
+  grad_code, _, grad_cols, grad_stride = matrix(grad, "grad", plan.tokens)
+  if grad_code != code or grad_cols != cols:
     raise invalid("grad and y need one type and width")
   w = _weights(weights, plan)
   grad_y, gy_stride = _output(grad_y, plan.pairs, cols, y, "grad_y")
   if grad_weights is None:
-    grad_weights = y.new_empty((plan.tokens, plan.topk), dtype=torch.float32)
+    grad_weights = y.new_empty(plan.tokens, plan.topk, dtype=torch.float32)
   C.check(C.lib.xse_expert_combine_backward(
       grad.data_ptr(), y.data_ptr(), code, cols, grad_stride, y_stride,
       plan.ref, w, grad_y.data_ptr(), gy_stride, _weights(grad_weights, plan),
@@ -231,13 +220,13 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
   in] in the tokens' order, or [tokens * topk, in] with sorted_rows; w holds
   num_experts groups of [out, in], bias is [num_experts, out]. out is
   [tokens * topk, out] of x's type by default."""
-  code = float_code(x, "x")
   index = x.get_device()
   if elsewhere(index, stream):
     with on(index, stream):
       return linear(x, plan, w, bias, activation, out,
                     sorted_rows=sorted_rows)
-  cols, stride = _rows(x, plan.pairs if sorted_rows else plan.tokens, "x")
+  code, _, cols, stride = matrix(
+      x, "x", plan.pairs if sorted_rows else plan.tokens)
   if cols != w.cols:
     raise invalid(f"x has {cols} columns, w {w.cols}")
   bias_ptr = bias_pointer(bias, (w.groups, w.rows))

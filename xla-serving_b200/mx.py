@@ -44,20 +44,24 @@ def float_code(t, what):
   return code
 
 
-def row_stride(t, what):
-  """Row stride of a 2-D tensor whose rows are contiguous."""
+def matrix(t, what, rows=None):
+  """(XSE_DT_*, rows, columns, row stride) of a 2-D float32 or bfloat16 CUDA
+  tensor whose rows are contiguous (and as many as `rows`, if given)."""
+  code = float_code(t, what)
   shape = t.shape
   if len(shape) != 2:
     raise invalid(f"{what} must be 2-D, got shape {tuple(shape)}")
-  rows, cols = shape
+  n, cols = shape
+  if rows is not None and n != rows:
+    raise invalid(f"{what} must have {rows} rows, got shape {tuple(shape)}")
   stride, step = t.stride()
   if cols > 1 and step != 1:
     raise invalid(f"{what} needs unit column stride")
-  if rows > 1:
-    if stride < cols:
-      raise invalid(f"{what} needs a row stride of at least its columns")
-    return stride
-  return max(cols, 1)
+  if n <= 1:
+    return code, n, cols, max(cols, 1)
+  if stride < cols:
+    raise invalid(f"{what} needs a row stride of at least its columns")
+  return code, n, cols, stride
 
 
 def elsewhere(index, stream):
@@ -70,6 +74,8 @@ def elsewhere(index, stream):
 def on(index, stream):
   """Makes a device and (if given) a stream of it current: the call's scratch
   and outputs then come from that stream's pool."""
+  if index < 0:
+    raise invalid("tensors must be on a CUDA device")
   if stream is not None and stream.device.index != index:
     raise invalid(f"a stream of {stream.device} for tensors on device {index}")
   with torch.cuda.device(index):
@@ -129,16 +135,18 @@ class MxMatrix:
   def get_device(self):
     return self._codes.get_device()
 
-  def new_empty(self, shape, dtype=torch.uint8):
+  dtype = torch.uint8
+
+  def new_empty(self, *shape, dtype=torch.uint8):
     """A tensor on the matrix's device."""
-    return self._codes.new_empty(shape, dtype=dtype)
+    return self._codes.new_empty(*shape, dtype=dtype)
 
   @classmethod
   def empty(cls, rows, cols, groups=1, device="cuda"):
     """A matrix to be filled; codes and scales share one allocation."""
-    if rows < 0 or rows >= 2 ** 31 or cols < 1 or groups < 1:
-      raise invalid("4-bit matrix needs 0 <= rows < 2^31, cols >= 1 and "
-                    "groups >= 1.")
+    if rows < 0 or rows >= 2 ** 31 or not 1 <= cols <= 2 ** 30 or groups < 1:
+      raise invalid("4-bit matrix needs 0 <= rows < 2^31, 1 <= cols <= 2^30 "
+                    "and groups >= 1.")
     at = groups * rows * ((cols + 31) // 32 * 16)  # a multiple of 16
     self = cls.__new__(cls)
     self._codes = torch.empty(
@@ -187,14 +195,15 @@ def dequantize(q: MxMatrix, out=None, *, dtype=torch.float32, stream=None):
       return dequantize(q, out, dtype=dtype)
   shape = (q.rows, q.cols) if q.groups == 1 else (q.groups, q.rows, q.cols)
   if out is None:
-    out = q.new_empty(shape, dtype)
+    out = q.new_empty(*shape, dtype=dtype)
   elif out.shape != shape:
     raise invalid(f"out has shape {tuple(out.shape)}, not {shape}")
-  code = float_code(out, "out")
   if q.groups == 1:
-    group_stride, stride = 0, row_stride(out, "out")
+    group_stride, (code, _, _, stride) = 0, matrix(out, "out")
   else:
-    group_stride, stride = out.stride(0), row_stride(out[0], "out")
+    group_stride, (code, _, _, stride) = out.stride(0), matrix(out[0], "out")
+    if group_stride == 0:
+      raise invalid("out's groups need places of their own")
   C.check(C.lib.xse_mxfp4_dequantize(q.ref, out.data_ptr(), code, group_stride,
                                      stride, current_stream(index, out)))
   return out
@@ -215,10 +224,13 @@ def layer_output(out, like, rows, cols, dtype):
   """(tensor, XSE_DT_*, row stride) of a layer's [rows, cols] output, a new one
   of `like`'s device without `out`."""
   if out is None:
-    return like.new_empty((rows, cols), dtype=dtype), _FLOATS[dtype], cols
+    if like.dtype == dtype:
+      return like.new_empty(rows, cols), _FLOATS[dtype], cols
+    return like.new_empty(rows, cols, dtype=dtype), _FLOATS[dtype], cols
   if out.shape != (rows, cols):
     raise invalid(f"out has shape {tuple(out.shape)}, not {(rows, cols)}")
-  return out, float_code(out, "out"), row_stride(out, "out")
+  code, _, _, stride = matrix(out, "out")
+  return out, code, stride
 
 
 def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
@@ -239,9 +251,7 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
         x.ref, w.ref, bias_ptr, activation, out.data_ptr(), out_code,
         out_stride, current_stream(index, x, bias, out)))
     return out
-  code = float_code(x, "x")
-  x_stride = row_stride(x, "x")
-  rows, cols = x.shape
+  code, rows, cols, x_stride = matrix(x, "x")
   if cols != w.cols:
     raise invalid(f"x has {cols} columns, w {w.cols}")
   out, out_code, out_stride = layer_output(out, x, rows, w.rows, x.dtype)
