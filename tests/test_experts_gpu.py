@@ -80,7 +80,8 @@ def make(rows, cols, dtype, seed):
 
 ROWS = [  # tokens, topk, experts, cols
     (1, 1, 1, 1), (3, 2, 4, 7), (64, 4, 64, 256), (50, 3, 5, 479),
-    (129, 8, 16, 1032), (1000, 2, 8, 64), (17, 6, 3, 4096)]
+    (129, 8, 16, 1032), (1000, 2, 8, 64), (17, 6, 3, 4096),
+    (20, 12, 30, 136), (9, 40, 50, 77), (3, 40, 64, 128)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -203,7 +204,8 @@ LAYERS = [  # tokens, topk, experts, in, out
     (1, 1, 1, 32, 16), (4, 2, 8, 64, 128), (64, 4, 16, 256, 200),
     (40, 2, 3, 479, 64), (300, 4, 4, 512, 256), (200, 8, 64, 100, 130),
     (1500, 2, 6, 320, 128), (2, 1, 256, 700, 40), (600, 1, 1, 96, 96),
-    (900, 2, 5, 1600, 270), (700, 1, 2, 2048, 128), (30, 2, 40, 9000, 140)]
+    (900, 2, 5, 1600, 270), (700, 1, 2, 2048, 128), (30, 2, 40, 9000, 140),
+    (100, 40, 50, 160, 64)]
 
 
 def expert_reference(x_rows, offsets, w, bias, act):
@@ -330,6 +332,51 @@ def test_mixture_of_experts(mx, experts, tokens, dtype):
   graph.replay()
   torch.cuda.synchronize()
   assert torch.equal(captured, mixture(mx, experts, *args)[-1])
+
+
+def test_plan_from_other_tensors(experts):
+  """A plan whose arrays lie on no 16-byte boundary, and one sorted into."""
+  tokens, topk, num_experts, cols = 50, 4, 6, 64
+  ids = torch.from_numpy(choose(tokens, topk, num_experts, seed=7)).cuda()
+  plan = experts.sort(ids, num_experts)
+  odd = lambda t: torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)  # noqa: E731
+  other = experts.ExpertPlan(odd(plan.offsets), odd(plan.order),
+                             odd(plan.slots))
+  assert other.slots.data_ptr() % 16 == 4
+  y = make(tokens * topk, cols, torch.float32, 1).cuda()
+  w = make(tokens, topk, torch.float32, 2).cuda()
+  assert torch.equal(experts.combine(y, other, w), experts.combine(y, plan, w))
+  other.slots.fill_(-7)
+  assert experts.sort(ids, num_experts, other) is other
+  for a, b in ((other.offsets, plan.offsets), (other.order, plan.order),
+               (other.slots, plan.slots)):
+    assert torch.equal(a, b)
+
+
+def test_offsets_past_32_bits(experts):
+  """Sorted rows more than 2^32 bytes apart."""
+  tokens, topk, num_experts, cols = 300_000, 8, 16, 1024
+  gen = torch.Generator(device="cuda").manual_seed(0)
+  ids = torch.randint(0, num_experts, (tokens, topk), generator=gen,
+                      device="cuda")
+  plan = experts.sort(ids, num_experts)
+  x = torch.randint(-8, 8, (tokens, cols), generator=gen, device="cuda",
+                    dtype=torch.int8).bfloat16()
+  rows = experts.gather(x, plan)
+  assert rows.numel() * 2 > 2 ** 32
+  some = torch.tensor([0, 1, 77_777, 2_100_000, 2_399_998, 2_399_999],
+                      device="cuda")
+  assert torch.equal(rows[some], x[plan.order[some].long() // topk])
+  back = experts.combine(rows, plan)  # topk times x: exact
+  assert torch.equal(back, x * topk)
+  gy, gw = experts.combine_backward(x, rows, plan, out_weights(plan))
+  assert torch.equal(gy[some], rows[some] * 2)
+  want = (x[-5:].double() ** 2).sum(1, keepdim=True).expand(-1, topk)
+  assert torch.equal(gw[-5:].double(), want)  # integers below 2^24
+
+
+def out_weights(plan):
+  return torch.full((plan.tokens, plan.topk), 2.0, device="cuda")
 
 
 def test_refusals(mx, experts, xse):

@@ -267,6 +267,26 @@ def test_linear_on_other_streams_and_in_graphs(mx):
       assert torch.equal(a, b)
 
 
+def test_offsets_past_32_bits(mx):
+  """More than 2^32 elements in x and in y."""
+  rows, cols = 70_000, 65_536
+  x = torch.empty((rows, cols), dtype=torch.bfloat16, device="cuda")
+  for part in x.split(10_000):
+    part.normal_()
+  q = mx.quantize(x)
+  back = mx.dequantize(q, dtype=torch.bfloat16)
+  for r in (0, 65_537, rows - 1):
+    np.testing.assert_array_equal(
+        back[r:r + 1].double().cpu().numpy(),
+        ref.quantized(x[r:r + 1].double().cpu().numpy()))
+  del x, q, back
+  w, _ = weights(mx, 32, 64)
+  x = make(40_000, 64, torch.float32, seed=8).cuda()
+  y = torch.empty((40_000, 110_000), device="cuda")[:, :32]
+  mx.linear(x, w, out=y)
+  assert torch.equal(y, mx.linear(x, w))
+
+
 def test_refusals(mx, xse):
   x = torch.zeros((4, 64), device="cuda")
   w, _ = weights(mx, 32, 64)
