@@ -19,7 +19,7 @@ import torch
 
 from . import _capi as C
 from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_stream, elsewhere,
-                 invalid, layer_output, matrix, on)
+                 invalid, layer_output, matrix, on, same_device)
 
 MAX_EXPERTS = 1024
 _INDEX = {torch.int32: C.INDEX_I32, torch.int64: C.INDEX_I64}
@@ -32,7 +32,7 @@ class ExpertPlan:
   a dropped one)."""
 
   __slots__ = ("_offsets", "_order", "_slots", "_buffer", "tokens", "topk",
-               "pairs", "num_experts", "ref")
+               "pairs", "num_experts", "shape", "index", "ref")
 
   def __init__(self, offsets, order, slots):
     for name, t in (("offsets", offsets), ("order", order), ("slots", slots)):
@@ -52,6 +52,8 @@ class ExpertPlan:
   def _set(self, offsets, order, slots, tokens, topk, num_experts):
     self.tokens, self.topk, self.num_experts = tokens, topk, num_experts
     self.pairs = tokens * topk
+    self.shape = (tokens, topk)  # of ids, slots and weights
+    self.index = self._buffer.get_device()
     self.ref = ctypes.byref(C.ExpertPlanStruct(offsets, order, slots, tokens,
                                                topk, num_experts))
 
@@ -82,7 +84,7 @@ class ExpertPlan:
     return self._buffer.device
 
   def get_device(self):
-    return self._buffer.get_device()
+    return self.index
 
   @classmethod
   def empty(cls, tokens, topk, num_experts, device="cuda"):
@@ -126,23 +128,23 @@ def sort(ids, num_experts, plan=None, *, stream=None) -> ExpertPlan:
   elif (plan.tokens, plan.topk, plan.num_experts) != (tokens, topk,
                                                       num_experts):
     raise invalid("the plan has other sizes than ids")
+  same_device(index, plan)
   size = C.lib.xse_expert_sort_workspace(plan.pairs, num_experts)
   scratch = ids.new_empty(size, dtype=torch.uint8) if size else None
   C.check(C.lib.xse_expert_sort(
       ids.data_ptr(), code, plan.ref, scratch.data_ptr() if size else None,
-      size, current_stream(index, plan)))
+      size, current_stream(index)))
   return plan
 
 
 def _weights(weights, plan):
   if weights is None:
     return None
-  if weights.dtype != torch.float32 or \
-      weights.shape != (plan.tokens, plan.topk) or \
+  if weights.dtype != torch.float32 or weights.shape != plan.shape or \
       not weights.is_contiguous():
-    raise invalid("weights must be contiguous float32 of shape "
-                  f"{(plan.tokens, plan.topk)}, got {weights.dtype} "
-                  f"{tuple(weights.shape)}")
+    raise invalid(f"weights must be contiguous float32 of shape {plan.shape}, "
+                  f"got {weights.dtype} {tuple(weights.shape)}")
+  same_device(plan.index, weights)
   return weights.data_ptr()
 
 
@@ -150,6 +152,7 @@ def _output(out, rows, cols, like, what="out"):
   """(tensor, row stride) of an output of `like`'s type."""
   if out is None:
     return like.new_empty(rows, cols), cols
+  same_device(like.get_device(), out)
   if out.shape != (rows, cols) or out.dtype != like.dtype:
     raise invalid(f"{what} must be {like.dtype} of shape {(rows, cols)}, got "
                   f"{out.dtype} {tuple(out.shape)}")
@@ -163,11 +166,13 @@ def gather(x, plan: ExpertPlan, out=None, *, stream=None):
   if elsewhere(index, stream):
     with on(index, stream):
       return gather(x, plan, out)
+  if plan.index != index:
+    same_device(index, plan)
   code, _, cols, stride = matrix(x, "x", plan.tokens)
   out, out_stride = _output(out, plan.pairs, cols, x)
   C.check(C.lib.xse_expert_gather(
       x.data_ptr(), code, cols, stride, plan.ref, out.data_ptr(), out_stride,
-      current_stream(index, plan, out)))
+      current_stream(index)))
   return out
 
 
@@ -179,12 +184,14 @@ def combine(y, plan: ExpertPlan, weights=None, out=None, *, stream=None):
   if elsewhere(index, stream):
     with on(index, stream):
       return combine(y, plan, weights, out)
+  if plan.index != index:
+    same_device(index, plan)
   code, _, cols, stride = matrix(y, "y", plan.pairs)
   w = _weights(weights, plan)
   out, out_stride = _output(out, plan.tokens, cols, y)
   C.check(C.lib.xse_expert_combine(
       y.data_ptr(), code, cols, stride, plan.ref, w, out.data_ptr(),
-      out_stride, current_stream(index, plan, weights, out)))
+      out_stride, current_stream(index)))
   return out
 
 
@@ -198,8 +205,11 @@ def combine_backward(grad, y, plan: ExpertPlan, weights=None, grad_y=None,
   if elsewhere(index, stream):
     with on(index, stream):
       return combine_backward(grad, y, plan, weights, grad_y, grad_weights)
+  if plan.index != index:
+    same_device(index, plan)
   code, _, cols, y_stride = matrix(y, "y", plan.pairs)
   grad_code, _, grad_cols, grad_stride = matrix(grad, "grad", plan.tokens)
+  same_device(index, grad)
   if grad_code != code or grad_cols != cols:
     raise invalid("grad and y need one type and width")
   w = _weights(weights, plan)
@@ -209,7 +219,7 @@ def combine_backward(grad, y, plan: ExpertPlan, weights=None, grad_y=None,
   C.check(C.lib.xse_expert_combine_backward(
       grad.data_ptr(), y.data_ptr(), code, cols, grad_stride, y_stride,
       plan.ref, w, grad_y.data_ptr(), gy_stride, _weights(grad_weights, plan),
-      current_stream(index, grad, plan, weights, grad_y, grad_weights)))
+      current_stream(index)))
   return grad_y, grad_weights
 
 
@@ -225,6 +235,7 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
     with on(index, stream):
       return linear(x, plan, w, bias, activation, out,
                     sorted_rows=sorted_rows)
+  same_device(index, plan, w, bias, out)
   code, _, cols, stride = matrix(
       x, "x", plan.pairs if sorted_rows else plan.tokens)
   if cols != w.cols:
@@ -237,5 +248,5 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
       x.data_ptr(), code, stride, 1 if sorted_rows else 0, plan.ref, w.ref,
       bias_ptr, activation, out.data_ptr(), out_code, out_stride,
       scratch.data_ptr() if size else None, size,
-      current_stream(index, plan, w, bias, out)))
+      current_stream(index)))
   return out

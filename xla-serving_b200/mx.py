@@ -86,13 +86,14 @@ def on(index, stream):
         yield
 
 
-def current_stream(index, *tensors):
-  """cudaStream_t of the current stream of device `index`, on which all the
-  call's tensors must lie."""
+current_stream = _raw_stream  # of a device's index: its cudaStream_t
+
+
+def same_device(index, *tensors):
+  """Refuses a call whose tensors do not all lie on device `index`."""
   for t in tensors:
     if t is not None and t.get_device() != index:
       raise invalid(f"tensors on {t.device} and device {index} in one call")
-  return _raw_stream(index)
 
 
 class MxMatrix:
@@ -100,7 +101,8 @@ class MxMatrix:
   scales are uint8 tensors of xse_mxfp4_codes_bytes and
   xse_mxfp4_scales_bytes."""
 
-  __slots__ = ("_codes", "_scales", "_at", "rows", "cols", "groups", "ref")
+  __slots__ = ("_codes", "_scales", "_at", "rows", "cols", "groups", "index",
+               "ref")
 
   def __init__(self, codes, scales, rows, cols, groups=1):
     for name, t, need in (
@@ -117,6 +119,7 @@ class MxMatrix:
 
   def _set(self, codes, scales, rows, cols, groups):
     self.rows, self.cols, self.groups = rows, cols, groups
+    self.index = self._codes.get_device()
     self.ref = ctypes.byref(C.MxMatrixStruct(codes, scales, rows, cols,
                                              groups))
 
@@ -133,7 +136,7 @@ class MxMatrix:
     return self._codes.device
 
   def get_device(self):
-    return self._codes.get_device()
+    return self.index
 
   dtype = torch.uint8
 
@@ -180,24 +183,28 @@ def quantize(x, out: Optional[MxMatrix] = None, *, stream=None) -> MxMatrix:
   elif (out.rows, out.cols, out.groups) != (rows, cols, groups):
     raise invalid(f"out holds {out.groups} x {out.rows} x {out.cols}, x has "
                   f"shape {tuple(shape)}")
+  if out.index != index:
+    same_device(index, out)
   C.check(C.lib.xse_mxfp4_quantize(
       x.data_ptr(), code, group_stride, strides[-2], strides[-1], out.ref,
-      current_stream(index, out)))
+      current_stream(index)))
   return out
 
 
 def dequantize(q: MxMatrix, out=None, *, dtype=torch.float32, stream=None):
   """The values q stands for, [rows, cols] ([groups, rows, cols] for several
   groups), in float32 or bfloat16 (exact in both)."""
-  index = q.get_device()
+  index = q.index
   if elsewhere(index, stream):
     with on(index, stream):
       return dequantize(q, out, dtype=dtype)
   shape = (q.rows, q.cols) if q.groups == 1 else (q.groups, q.rows, q.cols)
   if out is None:
     out = q.new_empty(*shape, dtype=dtype)
-  elif out.shape != shape:
-    raise invalid(f"out has shape {tuple(out.shape)}, not {shape}")
+  else:
+    same_device(index, out)
+    if out.shape != shape:
+      raise invalid(f"out has shape {tuple(out.shape)}, not {shape}")
   if q.groups == 1:
     group_stride, (code, _, _, stride) = 0, matrix(out, "out")
   else:
@@ -205,7 +212,7 @@ def dequantize(q: MxMatrix, out=None, *, dtype=torch.float32, stream=None):
     if group_stride == 0:
       raise invalid("out's groups need places of their own")
   C.check(C.lib.xse_mxfp4_dequantize(q.ref, out.data_ptr(), code, group_stride,
-                                     stride, current_stream(index, out)))
+                                     stride, current_stream(index)))
   return out
 
 
@@ -239,17 +246,18 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
   MxMatrix already quantised) and w [out, in]; Q is `quantize`. Accumulated
   in fp32 and rounded once to out's type (x's by default; float32 for an
   MxMatrix)."""
-  index = w.get_device()
+  index = w.index
   if elsewhere(index, stream):
     with on(index, stream):
       return linear(x, w, bias, activation, out)
+  same_device(index, x, bias, out)
   bias_ptr = bias_pointer(bias, (w.rows,))
   if isinstance(x, MxMatrix):
     out, out_code, out_stride = layer_output(out, w, x.rows, w.rows,
                                              torch.float32)
     C.check(C.lib.xse_linear_forward_mxfp4_q(
         x.ref, w.ref, bias_ptr, activation, out.data_ptr(), out_code,
-        out_stride, current_stream(index, x, bias, out)))
+        out_stride, current_stream(index)))
     return out
   code, rows, cols, x_stride = matrix(x, "x")
   if cols != w.cols:
@@ -260,7 +268,7 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
   C.check(C.lib.xse_linear_forward_mxfp4(
       x.data_ptr(), code, rows, x_stride, w.ref, bias_ptr, activation,
       out.data_ptr(), out_code, out_stride,
-      scratch.data_ptr() if size else None, size, current_stream(index, x, bias, out)))
+      scratch.data_ptr() if size else None, size, current_stream(index)))
   return out
 
 
