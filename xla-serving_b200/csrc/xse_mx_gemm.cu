@@ -975,6 +975,10 @@ struct Pair {
   static constexpr int kScaleColumns = 24;
   static_assert(kN + kStages * kScaleColumns <= 512, "tensor memory");
   static constexpr int kPart = kN / 2;
+  // A tile's MMAs take 128 rows where no more exist: a group's last tile.
+  __device__ static int RowsFor(const Tile& t) {
+    return t.rows <= kN / 2 ? kN / 2 : kN;
+  }
 };
 
 template <typename T>
@@ -1069,7 +1073,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           TmaLoad3Pair(at, &p.a, s * (kStageK / 2), m * kM, t.group, bar);
           TmaLoad2Pair(at + kABytes, &p.b, s * (kStageK / 2),
-                       static_cast<int>(t.row) + rank * (kN / 2), bar);
+                       static_cast<int>(t.row) + rank * (C::RowsFor(t) / 2),
+                       bar);
           TmaLoad2Pair(scales, &p.a_scale_map, 0, a_tile + 2 * s, bar);
           TmaLoad2Pair(scales + kScaleBytes, &p.b_scale_map, 0, b_tile + 2 * s,
                        bar);
@@ -1092,6 +1097,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true;
     for (int item = first_item; ok && item < items; item += item_step) {
+      const bool half_rows =
+          C::RowsFor(TileOf<kN>(p, p.m_pairs, item, tile_begin, row_begin)) <
+          kN;
       ok = BarrierWait(SharedAddress(&acc_empty_bar), acc_phase ^ 1, &failed);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
@@ -1120,8 +1128,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 4; ++j) {
             if (j * 64 >= left) break;
             MmaPair(tmem, a_desc + j * 2, b_desc + j * 2,
-                    InstructionDesc<kN, 2 * kM>(j & 1), a_col + (j >> 1) * 4,
-                    b_col + (j >> 1) * 8, s > 0 || j > 0);
+                    half_rows ? InstructionDesc<kN / 2, 2 * kM>(j & 1)
+                              : InstructionDesc<kN, 2 * kM>(j & 1),
+                    a_col + (j >> 1) * 4, b_col + (j >> 1) * 8,
+                    s > 0 || j > 0);
           }
           CommitPair(SharedAddress(empty_bar + stage));
         }
