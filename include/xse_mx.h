@@ -13,7 +13,8 @@
  *
  * These layers stand beside xse_dlrm.h's; the reference's tower runs its
  * Dense layers in fp32 under XLA (examples/dlrm/model_jce.py:107-138) and has
- * no counterpart. All buffers are memory of the current device; `stream` is a
+ * no counterpart. All buffers are memory of the current device, outputs
+ * without elements in common with inputs or the workspace; `stream` is a
  * cudaStream_t (NULL: the legacy default stream). Calls return after their
  * launches; status codes and xse_last_error() as in xse_emb.h. No call keeps
  * memory of its own, so calls on several streams or in captured graphs only

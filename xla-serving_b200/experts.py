@@ -10,18 +10,24 @@ A mixture of experts for one batch:
 
 `gather` gives the sorted rows themselves, for experts computed elsewhere;
 `combine_backward` and `combine` without weights are the gradients of
-`combine` and `gather`.
+`combine` and `gather`. Outputs may not share elements with inputs.
 """
 
 import ctypes
+import functools
 
 import torch
 
 from . import _capi as C
 from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_stream, elsewhere,
-                 invalid, layer_output, matrix, on, same_device)
+                 invalid, layer_output, matrix, new_like, on,
+                 same_device)
 
 MAX_EXPERTS = 1024
+_sort_workspace = functools.lru_cache(maxsize=1024)(
+    C.lib.xse_expert_sort_workspace)
+_linear_workspace = functools.lru_cache(maxsize=1024)(
+    C.lib.xse_expert_linear_workspace)
 _INDEX = {torch.int32: C.INDEX_I32, torch.int64: C.INDEX_I64}
 
 
@@ -88,15 +94,14 @@ class ExpertPlan:
 
   @classmethod
   def empty(cls, tokens, topk, num_experts, device="cuda"):
-    """A plan to be filled; its arrays (slots, order, offsets, each on a
-    16-byte boundary) share one allocation."""
+    """A plan to be filled, on a device or that of a tensor; its arrays (slots,
+    order, offsets, each on a 16-byte boundary) share one allocation."""
     if topk < 1 or not 1 <= num_experts <= MAX_EXPERTS:
       raise invalid(f"an expert plan needs topk >= 1 and 1 to {MAX_EXPERTS} "
                     "experts")
     part = _quads(tokens * topk)
     self = cls.__new__(cls)
-    self._buffer = torch.empty(2 * part + num_experts + 1, dtype=torch.int32,
-                               device=device)
+    self._buffer = new_like(device, 2 * part + num_experts + 1, torch.int32)
     self._offsets = self._order = self._slots = None
     start = self._buffer.data_ptr()
     self._set(start + 8 * part, start + 4 * part, start, tokens, topk,
@@ -124,12 +129,12 @@ def sort(ids, num_experts, plan=None, *, stream=None) -> ExpertPlan:
       return sort(ids, num_experts, plan)
   tokens, topk = ids.shape
   if plan is None:
-    plan = ExpertPlan.empty(tokens, topk, num_experts, ids.device)
+    plan = ExpertPlan.empty(tokens, topk, num_experts, ids)
   elif (plan.tokens, plan.topk, plan.num_experts) != (tokens, topk,
                                                       num_experts):
     raise invalid("the plan has other sizes than ids")
   same_device(index, plan)
-  size = C.lib.xse_expert_sort_workspace(plan.pairs, num_experts)
+  size = _sort_workspace(plan.pairs, num_experts)
   scratch = ids.new_empty(size, dtype=torch.uint8) if size else None
   C.check(C.lib.xse_expert_sort(
       ids.data_ptr(), code, plan.ref, scratch.data_ptr() if size else None,
@@ -242,7 +247,7 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
     raise invalid(f"x has {cols} columns, w {w.cols}")
   bias_ptr = bias_pointer(bias, (w.groups, w.rows))
   out, out_code, out_stride = layer_output(out, x, plan.pairs, w.rows, x.dtype)
-  size = C.lib.xse_expert_linear_workspace(plan.pairs, plan.num_experts, cols)
+  size = _linear_workspace(plan.pairs, plan.num_experts, cols)
   scratch = w.new_empty(size) if size else None
   C.check(C.lib.xse_expert_linear_mxfp4(
       x.data_ptr(), code, stride, 1 if sorted_rows else 0, plan.ref, w.ref,

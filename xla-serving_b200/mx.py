@@ -10,6 +10,7 @@ and streams.
 
 import contextlib
 import ctypes
+import functools
 from typing import Optional
 
 import torch
@@ -22,6 +23,10 @@ BLOCK = 32  # elements per scale
 
 _FLOATS = {torch.float32: C.DT_F32, torch.bfloat16: C.DT_BF16}
 
+
+# Scratch bytes by sizes (a call into the library costs half a microsecond).
+_linear_workspace = functools.lru_cache(maxsize=1024)(
+    C.lib.xse_linear_mxfp4_workspace)
 
 # The current device's index and the raw cudaStream_t of a device's current
 # stream, without building torch objects: a call on a few rows lasts a few
@@ -62,6 +67,13 @@ def matrix(t, what, rows=None):
   if stride < cols:
     raise invalid(f"{what} needs a row stride of at least its columns")
   return code, n, cols, stride
+
+
+def new_like(device, size, dtype):
+  """`size` elements on a device, or on that of a tensor."""
+  if isinstance(device, torch.Tensor):
+    return device.new_empty(size, dtype=dtype)
+  return torch.empty(size, dtype=dtype, device=device)
 
 
 def elsewhere(index, stream):
@@ -146,15 +158,15 @@ class MxMatrix:
 
   @classmethod
   def empty(cls, rows, cols, groups=1, device="cuda"):
-    """A matrix to be filled; codes and scales share one allocation."""
+    """A matrix to be filled, on a device or that of a tensor; codes and scales
+    share one allocation."""
     if rows < 0 or rows >= 2 ** 31 or not 1 <= cols <= 2 ** 30 or groups < 1:
       raise invalid("4-bit matrix needs 0 <= rows < 2^31, 1 <= cols <= 2^30 "
                     "and groups >= 1.")
     at = groups * rows * ((cols + 31) // 32 * 16)  # a multiple of 16
     self = cls.__new__(cls)
-    self._codes = torch.empty(
-        at + groups * ((rows + 127) // 128) * ((cols + 127) // 128) * 512,
-        dtype=torch.uint8, device=device)
+    size = at + groups * ((rows + 127) // 128) * ((cols + 127) // 128) * 512
+    self._codes = new_like(device, size, torch.uint8)
     self._scales, self._at = None, at
     start = self._codes.data_ptr()
     self._set(start, start + at if start else 0, rows, cols, groups)
@@ -179,7 +191,7 @@ def quantize(x, out: Optional[MxMatrix] = None, *, stream=None) -> MxMatrix:
   else:
     raise invalid(f"x must be 2-D or 3-D, got shape {tuple(shape)}")
   if out is None:
-    out = MxMatrix.empty(rows, cols, groups, x.device)
+    out = MxMatrix.empty(rows, cols, groups, x)
   elif (out.rows, out.cols, out.groups) != (rows, cols, groups):
     raise invalid(f"out holds {out.groups} x {out.rows} x {out.cols}, x has "
                   f"shape {tuple(shape)}")
@@ -245,7 +257,7 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
   """out = act(Q(x) W^T + bias) for x [rows, in] (float32 or bfloat16, or an
   MxMatrix already quantised) and w [out, in]; Q is `quantize`. Accumulated
   in fp32 and rounded once to out's type (x's by default; float32 for an
-  MxMatrix)."""
+  MxMatrix). out may not share elements with x."""
   index = w.index
   if elsewhere(index, stream):
     with on(index, stream):
@@ -263,7 +275,7 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
   if cols != w.cols:
     raise invalid(f"x has {cols} columns, w {w.cols}")
   out, out_code, out_stride = layer_output(out, x, rows, w.rows, x.dtype)
-  size = C.lib.xse_linear_mxfp4_workspace(rows, cols)
+  size = _linear_workspace(rows, cols)
   scratch = w.new_empty(size) if size else None
   C.check(C.lib.xse_linear_forward_mxfp4(
       x.data_ptr(), code, rows, x_stride, w.ref, bias_ptr, activation,
