@@ -68,8 +68,8 @@ int RowShift(int64_t chunks) {
 }
 
 // `per_sm` blocks at most for each SM. The aligned quantisation runs best in one
-// wave of the six that its registers allow (8192 x 4096 fp32: 25 us, 28 us with
-// eight); the kernels that turn their elements with eight, whose second wave
+// wave of the six (to several places: five) that its registers allow (8192 x
+// 4096 fp32: 25 us, 28 us with eight); the kernels that turn their elements with eight, whose second wave
 // fills the first one's waits (read-back of the same: 29 us, 32 us with six).
 int BlocksForRows(int64_t rows, int row_shift, int per_sm) {
   const int64_t per = 1 << (kWarpShift - row_shift);
@@ -488,7 +488,8 @@ void LaunchQuantizeRows(QuantParams p, cudaStream_t s) {
   constexpr int kSpan = 32 * PartOf<T, kAligned>::kElements;
   p.row_shift = RowShift((p.k_tiles * 128 + kSpan - 1) / kSpan);
   QuantizeKernel<T, kMode, kAligned>
-      <<<BlocksForRows(p.total_rows, p.row_shift, kAligned ? 6 : 8), kThreads,
+      <<<BlocksForRows(p.total_rows, p.row_shift,
+                        !kAligned ? 8 : kMode == kFromTokens ? 5 : 6), kThreads,
          0, s>>>(p);
 }
 
