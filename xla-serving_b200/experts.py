@@ -19,8 +19,8 @@ import functools
 import torch
 
 from . import _capi as C
-from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_stream, elsewhere,
-                 invalid, layer_output, matrix, new_like, on,
+from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_device,
+                 current_stream, invalid, layer_output, matrix, new_like, on,
                  same_device)
 
 MAX_EXPERTS = 1024
@@ -124,7 +124,7 @@ def sort(ids, num_experts, plan=None, *, stream=None) -> ExpertPlan:
     raise invalid("expert ids must be a contiguous 2-D int32 or int64 CUDA "
                   f"tensor, got {ids.dtype} {tuple(ids.shape)}")
   index = ids.get_device()
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return sort(ids, num_experts, plan)
   tokens, topk = ids.shape
@@ -149,7 +149,8 @@ def _weights(weights, plan):
       not weights.is_contiguous():
     raise invalid(f"weights must be contiguous float32 of shape {plan.shape}, "
                   f"got {weights.dtype} {tuple(weights.shape)}")
-  same_device(plan.index, weights)
+  if weights.get_device() != plan.index:
+    same_device(plan.index, weights)
   return weights.data_ptr()
 
 
@@ -168,7 +169,7 @@ def gather(x, plan: ExpertPlan, out=None, *, stream=None):
   """x's rows in sorted order: out[r] = x[plan.order[r] // topk], zeros behind
   the last sorted row. Its gradient is combine(grad, plan)."""
   index = x.get_device()
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return gather(x, plan, out)
   if plan.index != index:
@@ -186,7 +187,7 @@ def combine(y, plan: ExpertPlan, weights=None, out=None, *, stream=None):
   without them), summed in fp32 in the order of the choices; a row all of
   whose pairs were dropped is zero."""
   index = y.get_device()
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return combine(y, plan, weights, out)
   if plan.index != index:
@@ -207,7 +208,7 @@ def combine_backward(grad, y, plan: ExpertPlan, weights=None, grad_y=None,
   (t, j) the dot product of grad[t] and its sorted row (0 for a dropped
   pair)."""
   index = y.get_device()
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return combine_backward(grad, y, plan, weights, grad_y, grad_weights)
   if plan.index != index:
@@ -236,7 +237,7 @@ def linear(x, plan: ExpertPlan, w: MxMatrix, bias=None, activation=ACT_NONE,
   num_experts groups of [out, in], bias is [num_experts, out]. out is
   [tokens * topk, out] of x's type by default."""
   index = x.get_device()
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return linear(x, plan, w, bias, activation, out,
                     sorted_rows=sorted_rows)

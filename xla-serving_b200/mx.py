@@ -31,8 +31,8 @@ _linear_workspace = functools.lru_cache(maxsize=1024)(
 # The current device's index and the raw cudaStream_t of a device's current
 # stream, without building torch objects: a call on a few rows lasts a few
 # microseconds, as long as those would take.
-_current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
-_raw_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
+current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
+current_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
 
 
 def invalid(message):
@@ -76,15 +76,10 @@ def new_like(device, size, dtype):
   return torch.empty(size, dtype=dtype, device=device)
 
 
-def elsewhere(index, stream):
-  """Whether a call on device `index` has to change the current device or
-  stream first (it is then made again within `on`)."""
-  return stream is not None or index != _current_device()
-
-
 @contextlib.contextmanager
 def on(index, stream):
-  """Makes a device and (if given) a stream of it current: the call's scratch
+  """Makes a device and (if given) a stream of it current. A call for another
+  device or stream than the current ones makes itself again within: its scratch
   and outputs then come from that stream's pool."""
   if index < 0:
     raise invalid("tensors must be on a CUDA device")
@@ -96,9 +91,6 @@ def on(index, stream):
     else:
       with torch.cuda.stream(stream):
         yield
-
-
-current_stream = _raw_stream  # of a device's index: its cudaStream_t
 
 
 def same_device(index, *tensors):
@@ -179,7 +171,7 @@ def quantize(x, out: Optional[MxMatrix] = None, *, stream=None) -> MxMatrix:
   [in, out] kernel is quantised as `quantize(kernel.t())`."""
   code = float_code(x, "x")
   index = x.get_device()
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return quantize(x, out)
   shape, strides = x.shape, x.stride()
@@ -207,7 +199,7 @@ def dequantize(q: MxMatrix, out=None, *, dtype=torch.float32, stream=None):
   """The values q stands for, [rows, cols] ([groups, rows, cols] for several
   groups), in float32 or bfloat16 (exact in both)."""
   index = q.index
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return dequantize(q, out, dtype=dtype)
   shape = (q.rows, q.cols) if q.groups == 1 else (q.groups, q.rows, q.cols)
@@ -259,7 +251,7 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
   in fp32 and rounded once to out's type (x's by default; float32 for an
   MxMatrix). out may not share elements with x."""
   index = w.index
-  if elsewhere(index, stream):
+  if stream is not None or index != current_device():
     with on(index, stream):
       return linear(x, w, bias, activation, out)
   same_device(index, x, bias, out)
