@@ -334,6 +334,34 @@ def test_mixture_of_experts(mx, experts, tokens, dtype):
   assert torch.equal(captured, mixture(mx, experts, *args)[-1])
 
 
+def test_empty_batch(mx, experts):
+  """No tokens: every call returns its empty outputs."""
+  plan = experts.sort(torch.zeros((0, 3), dtype=torch.int64, device="cuda"), 5)
+  x = torch.zeros((0, 64), device="cuda")
+  w, _ = expert_weights(mx, 5, 32, 64)
+  weights = torch.zeros((0, 3), device="cuda")
+  assert experts.gather(x, plan).shape == (0, 64)
+  assert experts.combine(x, plan, weights).shape == (0, 64)
+  assert experts.linear(x, plan, w).shape == (0, 32)
+  gy, gw = experts.combine_backward(x, x, plan, weights)
+  assert gy.shape == (0, 64) and gw.shape == (0, 3)
+
+
+@pytest.mark.parametrize("tokens", [6, 200])
+def test_rows_off_the_16_byte_grid(mx, experts, tokens):
+  """Rows that begin off the grid give the numbers of rows on it."""
+  topk, num_experts, cols = 2, 4, 200
+  ids = choose(tokens, topk, num_experts, seed=8)
+  plan = experts.sort(torch.from_numpy(ids).cuda(), num_experts)
+  w, _ = expert_weights(mx, num_experts, 40, cols)
+  for dtype in (torch.float32, torch.bfloat16):
+    x = make(tokens, cols, dtype, 1).cuda()
+    buf = torch.zeros((tokens, cols + 9), dtype=dtype, device="cuda")
+    buf[:, 3:3 + cols] = x
+    assert torch.equal(experts.linear(buf[:, 3:3 + cols], plan, w),
+                       experts.linear(x, plan, w))
+
+
 def test_plan_from_other_tensors(experts):
   """A plan whose arrays lie on no 16-byte boundary, and one sorted into."""
   tokens, topk, num_experts, cols = 50, 4, 6, 64
