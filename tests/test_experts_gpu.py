@@ -362,6 +362,30 @@ def test_rows_off_the_16_byte_grid(mx, experts, tokens):
                        experts.linear(x, plan, w))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("cols,pad", [
+    (1024, 1), (1025, 0), (1025, 2), (1500, 3), (2047, 4), (2048, 1),
+    (2049, 0), (4099, 6)])
+@pytest.mark.parametrize("tokens,topk", [(1, 1), (37, 3), (1300, 9)])
+def test_gather_long_rows_off_the_grid(experts, tokens, topk, cols, pad,
+                                       dtype):
+  """Long rows that begin at any element: the bits of x, zeros behind the last
+  sorted row, and what lies between the rows of `out` as it was."""
+  num_experts = 5
+  ids = choose(tokens, topk, num_experts, seed=9)
+  plan = experts.sort(torch.from_numpy(ids).cuda(), num_experts)
+  order = plan.order.long()
+  wide = cols + 2 * pad + 1
+  source = make(tokens, wide, dtype, 4).cuda()
+  x = source[:, pad:pad + cols]
+  store = torch.full((tokens * topk, wide), 7.0, dtype=dtype, device="cuda")
+  want = store.clone()
+  want[:, pad + 1:pad + 1 + cols] = torch.where(
+      (order >= 0)[:, None], x[order.clamp(min=0) // topk], 0.0).to(dtype)
+  experts.gather(x, plan, out=store[:, pad + 1:pad + 1 + cols])
+  assert torch.equal(store, want)
+
+
 def test_plan_from_other_tensors(experts):
   """A plan whose arrays lie on no 16-byte boundary, and one sorted into."""
   tokens, topk, num_experts, cols = 50, 4, 6, 64

@@ -785,6 +785,69 @@ __global__ void __launch_bounds__(kThreads)
   ZeroTail<T, 1>(p);
 }
 
+// The gather of long rows at any alignment goes through shared memory: a block
+// loads a piece of a token's row once and writes it to each of its sorted rows
+// in whole 128-byte lines of the destination (ragged at the piece's ends),
+// 4 bytes a thread, where single elements that follow the source's lines touch
+// two lines a warp and half of each word in 16 bits. Taken for rows of more
+// than kWide * kThreads elements, which a block of GatherElementsKernel needs
+// several steps for; against it, 16384 tokens x 4: 92 us for 162 at 1501 fp32,
+// 129 for 215 at 2047, 90 for 121 at 2047 bf16. Shorter rows leave most of a
+// block idle between its barriers: 62 us for 42 at 511 fp32, 65 for 67 at 1001
+// bf16.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    GatherPiecesKernel(const __grid_constant__ MoveParams p) {
+  constexpr int kPieceElements = 2048, kPer = kPieceElements / kThreads;
+  constexpr int kWord = 4 / sizeof(T);  // elements of a word
+  __shared__ T piece[kPieceElements];
+  for (int64_t t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    const T* x = static_cast<const T*>(p.src) + t * p.src_stride;
+    for (int first = 0; first < p.cols; first += kPieceElements) {
+      const int count = min(p.cols - first, kPieceElements);
+      T v[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int c = i * kThreads + threadIdx.x;
+        if (c < count) v[i] = x[first + c];
+      }
+      __syncthreads();  // the last piece has been written
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int c = i * kThreads + threadIdx.x;
+        if (c < count) piece[c] = v[i];
+      }
+      __syncthreads();
+      for (int j = 0; j < p.topk; ++j) {
+        const int32_t slot = SlotOf(p, t, j);
+        if (!Kept(p, slot)) continue;
+        T* dst = static_cast<T*>(p.dst) + slot * p.dst_stride + first;
+        // Elements from the last line boundary to the first one of the piece.
+        const int ahead = static_cast<int>(
+            (reinterpret_cast<uintptr_t>(dst) & 127) / sizeof(T));
+        for (int e = static_cast<int>(threadIdx.x) * kWord - ahead; e < count;
+             e += kThreads * kWord) {
+          if constexpr (kWord == 1) {
+            if (e >= 0) dst[e] = piece[e];
+          } else if (e >= 0 && e + 1 < count) {
+            Piece<T, 2> two;
+            two.v[0] = piece[e];
+            two.v[1] = piece[e + 1];
+            uint32_t w;
+            __builtin_memcpy(&w, &two, 4);
+            *reinterpret_cast<uint32_t*>(dst + e) = w;
+          } else if (e >= 0) {
+            dst[e] = piece[e];
+          } else if (e + 1 >= 0) {
+            dst[e + 1] = piece[e + 1];
+          }
+        }
+      }
+    }
+  }
+  ZeroTail<T, 1>(p);
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     CombineElementsKernel(const __grid_constant__ MoveParams p) {
@@ -967,7 +1030,9 @@ cudaError_t LaunchMove(int op, MoveParams p, bool vec, cudaStream_t s) {
   } else {
     p.row_shift = ThreadShift((p.cols + kWide - 1) / kWide, kThreads);
     const int blocks = Blocks(p.tokens, kThreads >> p.row_shift, 8);
-    if (op == kGather) {
+    if (op == kGather && p.cols > kWide * kThreads) {
+      GatherPiecesKernel<T><<<Blocks(p.tokens, 1, 8), kThreads, 0, s>>>(p);
+    } else if (op == kGather) {
       GatherElementsKernel<T><<<blocks, kThreads, 0, s>>>(p);
     } else {
       CombineElementsKernel<T><<<blocks, kThreads, 0, s>>>(p);
