@@ -998,7 +998,7 @@ cudaError_t LaunchRing(int op, MoveParams p, cudaStream_t s) {
   const auto kernel = op == kCombine ? CombineRingKernel<T, kC>
                                      : CombineBackwardRingKernel<T, kC>;
   p.row_shift = ThreadShift(p.cols / (16 / static_cast<int>(sizeof(T))),
-                            op == kCombine ? 256 : 32);
+                            op == kCombine ? kRingRowThreads : 32);
   const cudaError_t e =
       AllowShared(kernel, kRingBytes, &allowed[op == kCombine]);
   if (e != cudaSuccess) return e;
@@ -1049,7 +1049,8 @@ cudaError_t LaunchMoveAs(int op, MoveParams p, cudaStream_t s) {
                    Aligned16(p.dst) && p.src_stride % kV == 0 &&
                    p.y_stride % kV == 0 && p.dst_stride % kV == 0 &&
                    p.src_stride < kMost && p.y_stride < kMost &&
-                   p.dst_stride < kMost;
+                   p.dst_stride < kMost &&
+                   (op == kGather || ExpertRowFitsRing(p.cols, sizeof(T)));
   p.src_bytes = static_cast<uint32_t>(p.src_stride * sizeof(T));
   p.y_bytes = static_cast<uint32_t>(p.y_stride * sizeof(T));
   p.dst_bytes = static_cast<uint32_t>(p.dst_stride * sizeof(T));

@@ -92,6 +92,16 @@ inline bool MxQuantizesInProduct(int n, int32_t k) {
              kRowBufferBytes;
 }
 
+// Whether expert rows of `cols` elements of `size` bytes may go through the ring
+// kernels, which count a row's bytes in 32 bits: the offset after the row's
+// last 16-byte pieces, a step of all the threads that share a row further on,
+// still has to fit. Wider rows (fp32 within 4 KB of 4 GB, which xse_experts.h
+// allows) go element by element.
+constexpr int kRingRowThreads = 256;  // that share a row at most
+constexpr bool ExpertRowFitsRing(int64_t cols, int64_t size) {
+  return cols * size <= UINT32_MAX - kRingRowThreads * 16;
+}
+
 // Quantises the rows of x for a product in tiles of `tile_rows`: plan NULL, one
 // group as xse_mxfp4_quantize lays it out; else to the sorted rows' places
 // (codes by sorted row, scales as ExpertScaleTiles says), from token rows or
