@@ -287,6 +287,27 @@ def test_offsets_past_32_bits(mx):
   assert torch.equal(y, mx.linear(x, w))
 
 
+def test_row_whose_scales_pass_32_bits(mx):
+  """A row of more than 2^29 columns: its scale tiles take more than 2^31
+  bytes. Blocks do not depend on one another, so shorter rows give its values."""
+  cols, short = 2 ** 29 + 4096, 4096
+  x = torch.empty((1, cols), dtype=torch.bfloat16, device="cuda")
+  gen = torch.Generator(device="cuda").manual_seed(0)
+  for part in x.view(-1).split(2 ** 26):
+    part.normal_(generator=gen)
+  want = mx.dequantize(mx.quantize(x.view(-1, short)), dtype=x.dtype)
+  q = mx.quantize(x)
+  assert q.scales.numel() > 2 ** 31
+  got = mx.dequantize(q, dtype=x.dtype)
+  assert torch.equal(got.view(-1, short), want)
+  np.testing.assert_array_equal(
+      got[:, -short:].double().cpu().numpy(),
+      ref.quantized(x[:, -short:].double().cpu().numpy()))
+  odd = torch.empty((1, cols + 1), device="cuda")[:, 1:]  # off the 16-byte grid
+  mx.dequantize(q, odd)
+  assert torch.equal(odd, got.float())
+
+
 def test_refusals(mx, xse):
   x = torch.zeros((4, 64), device="cuda")
   w, _ = weights(mx, 32, 64)

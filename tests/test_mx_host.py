@@ -18,6 +18,8 @@ int main(int, char** argv) {
   const long long cols = atoll(argv[1]), size = atoll(argv[2]);
   printf("ring %d\n", xse::ExpertRowFitsRing(cols, size) ? 1 : 0);
   printf("threads %d\n", xse::kRingRowThreads);
+  printf("scale %lld\n", static_cast<long long>(
+      xse::MxColumnScaleAt(static_cast<int>(cols))));
 }
 """
 
@@ -65,3 +67,11 @@ def test_ring_rows_end(host, cols, size):
   assert got["ring"] == (cols * size < 2 ** 32 - 4096)
   if not all(walk_ends(cols, size, t) for t in (32, 256)):
     assert not got["ring"]
+
+
+@pytest.mark.parametrize("col", [
+    0, 31, 32, 127, 128, 4096, 2 ** 29 - 1, 2 ** 29, 2 ** 29 + 96,
+    2 ** 30 - 1])
+def test_scale_of_a_far_column(host, col):
+  """The scale's place by the layout of include/xse_mx.h, past 2^31 bytes too."""
+  assert host(col, 4)["scale"] == col // 128 * 512 + col // 32 % 4

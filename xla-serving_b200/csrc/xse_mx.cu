@@ -434,7 +434,7 @@ __global__ void __launch_bounds__(kThreads)
         if (col < cols) {
           word[h] = __ldg(reinterpret_cast<const uint32_t*>(
               codes + row * row_bytes + col / 2));
-          s[h] = __ldg(row_scales + col / 128 * kMxTileBytes + col / 32 % 4);
+          s[h] = __ldg(row_scales + MxColumnScaleAt(col));
         }
       }
 #pragma unroll

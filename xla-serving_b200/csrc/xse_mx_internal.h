@@ -111,6 +111,12 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
                  int tile_rows, void* codes, void* scales,
                  cudaStream_t stream);
 
+// Byte offset of the scale of column `col` from that of its row's first block.
+// 64 bits: a row's scale tiles pass 2^31 bytes from 2^29 columns on.
+__host__ __device__ constexpr int64_t MxColumnScaleAt(int32_t col) {
+  return static_cast<int64_t>(col / 128) * kMxTileBytes + col / 32 % 4;
+}
+
 #ifdef __CUDACC__
 
 // The E8M0 byte of a block whose largest magnitude has these bits.
