@@ -254,7 +254,10 @@ class DenseTower:
     if split is not None and x.stride(0) != layer.kernel.shape[0]:
       split = None  # the split buffers are dense [rows, in]
     if split is None:
-      math = C.MATH_FP32 if self.math >= MATH_TF32X3 else self.math
+      # The tower's own modes leave such layers in fp32; others are the
+      # library's to take or refuse.
+      math = (C.MATH_FP32 if self.math in (MATH_TF32X3, MATH_MXFP4)
+              else self.math)
       return linear(x, layer, out, math=math, stream=stream)
     rows, width = x.shape[0], layer.kernel.shape[0]
     hi = bufs["hi"][:rows * width].view(rows, width)
