@@ -277,5 +277,10 @@ def linear(x, w: MxMatrix, bias=None, activation=ACT_NONE, out=None, *,
 
 
 def check(stream=None):
-  """Waits for the stream; raises if a product's kernel gave up a wait."""
-  C.check(C.lib.xse_mxfp4_check(stream_handle(stream)))
+  """Waits for the stream (the current one by default); raises if a product's
+  kernel on its device gave up a wait."""
+  if stream is None:
+    C.check(C.lib.xse_mxfp4_check(stream_handle()))
+    return
+  with torch.cuda.device(stream.device):
+    C.check(C.lib.xse_mxfp4_check(stream_handle(stream)))
