@@ -1,5 +1,6 @@
-"""mx.check on the CPU, with a device switch and a library that record: the
-failure flag is read on the stream's own device."""
+"""mx.check and its callers on the CPU, with a device switch and a library that
+record: the failure flag is read on the stream's own device, and a forward of
+4-bit layers reports it where it reports the lookup's errors."""
 
 import contextlib
 import types
@@ -49,3 +50,42 @@ def test_check_raises(xse, calls):
     with pytest.raises(xse.XseError) as e:
       xse.mx.check(stream)
     assert e.value.code == xse._capi.DEADLINE_EXCEEDED
+
+
+def forward(xse, monkeypatch, math, fused, status):
+  """A DLRM forward whose launches do nothing."""
+  engine = types.SimpleNamespace(
+      execute_interaction=lambda *args, **kwargs: None,
+      execute_batch=lambda *args, **kwargs: None)
+  for name in ("bottom_forward", "top_forward", "forward"):
+    monkeypatch.setattr(xse.dlrm.DenseTower, name,
+                        lambda *args, **kwargs: torch.zeros(3))
+  model = xse.dlrm.DLRM(engine, ["a", "b"], dim=128, device="cpu",
+                        fused_interaction=fused)
+  model.tower.math = math
+  model.forward(torch.zeros(3, 13), requests=[], status=status)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_status_of_a_forward_in_4_bits(xse, monkeypatch, calls, fused):
+  C, dlrm = xse._capi, xse.dlrm
+  found = types.SimpleNamespace(rc=C.OK)
+  monkeypatch.setattr(C.lib, "xse_status_create", lambda *args: C.OK)
+  monkeypatch.setattr(C.lib, "xse_status_wait", lambda *args: found.rc)
+  status = xse.Status()
+  stream = stream_of(1, 11)
+  calls.rc = C.DEADLINE_EXCEEDED
+  forward(xse, monkeypatch, C.MATH_FP32, fused, status)
+  status.wait(stream)  # no 4-bit product: nothing to ask
+  assert not calls.seen
+  forward(xse, monkeypatch, dlrm.MATH_MXFP4, fused, status)
+  found.rc = C.INVALID_ARGUMENT  # the lookup's own error comes first
+  with pytest.raises(xse.XseError) as e:
+    status.wait(stream)
+  assert e.value.code == C.INVALID_ARGUMENT and not calls.seen
+  found.rc = C.OK
+  with pytest.raises(xse.XseError) as e:
+    status.wait(stream)
+  assert e.value.code == C.DEADLINE_EXCEEDED and calls.seen == [(1, 11)]
+  status.wait(stream)  # asked once
+  assert calls.seen == [(1, 11)]

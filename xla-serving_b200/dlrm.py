@@ -174,7 +174,8 @@ class DenseTower:
 
   def forward(self, dense, pooled, *, stream=None):
     """dense [B, num_dense] fp32, pooled [B, T, dim] fp32 (a sample's T rows
-    contiguous) -> predictions [B] (a view of an internal buffer)."""
+    contiguous) -> predictions [B] (a view of an internal buffer). mx.check()
+    tells whether the products of MATH_MXFP4 are complete."""
     x = self.bottom_forward(dense, stream=stream)
     inter = self.interaction_buffer(dense.shape[0])
     C.check(C.lib.xse_dot_interaction_strided(
@@ -326,7 +327,12 @@ class DLRM:
   def forward(self, dense, ids=None, offsets=None, weights=None, *,
               requests=None, status: Optional[Status] = None, stream=None):
     """Predictions [B] for dense features [B, num_dense] and per-feature CSR
-    ids/offsets (or prebuilt `requests` from requests())."""
+    ids/offsets (or prebuilt `requests` from requests()).
+
+    With MATH_MXFP4 a product whose kernel gave up a wait leaves predictions
+    incomplete: status.wait() reports it; without `status`, mx.check() does."""
+    if status is not None and self.tower.math == MATH_MXFP4:
+      status.also(mx.check)
     if requests is None:
       requests, pooled = self.requests(ids, offsets, weights)
     else:

@@ -88,14 +88,22 @@ class Status:
 
   def __init__(self, max_requests=256):
     self._handle = ctypes.c_void_p()
+    self._also = None
     C.check(C.lib.xse_status_create(max_requests, ctypes.byref(self._handle)))
 
   @property
   def handle(self):
     return self._handle
 
+  def also(self, check):
+    """Has the next wait() that finds no error call check(stream) too."""
+    self._also = check
+
   def wait(self, stream=None):
     C.check(C.lib.xse_status_wait(self._handle, stream_handle(stream)))
+    if self._also is not None:
+      check, self._also = self._also, None
+      check(stream)
 
   def close(self):
     if self._handle:
