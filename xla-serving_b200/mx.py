@@ -30,9 +30,13 @@ _linear_workspace = functools.lru_cache(maxsize=1024)(
 
 # The current device's index and the raw cudaStream_t of a device's current
 # stream, without building torch objects: a call on a few rows lasts a few
-# microseconds, as long as those would take.
-current_device = torch._C._cuda_getDevice  # pylint: disable=protected-access
-current_stream = torch._C._cuda_getCurrentRawStream  # pylint: disable=protected-access
+# microseconds, as long as those would take. A torch without these (one without
+# CUDA, on which the package's host side still imports) has the public ones.
+current_device = getattr(torch._C, "_cuda_getDevice",  # pylint: disable=protected-access
+                         torch.cuda.current_device)
+current_stream = getattr(torch._C, "_cuda_getCurrentRawStream",  # pylint: disable=protected-access
+                         lambda index: torch.cuda.current_stream(
+                             index).cuda_stream)
 
 
 def invalid(message):
