@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _capi as C
-from .mx import (ACT_NONE, MxMatrix, bias_pointer, current_device,
+from .mx import (ACT_NONE, MOST_INT, MxMatrix, bias_pointer, current_device,
                  current_stream, invalid, layer_output, matrix, new_like, on,
                  same_device)
 
@@ -29,6 +29,15 @@ _sort_workspace = functools.lru_cache(maxsize=1024)(
 _linear_workspace = functools.lru_cache(maxsize=1024)(
     C.lib.xse_expert_linear_workspace)
 _INDEX = {torch.int32: C.INDEX_I32, torch.int64: C.INDEX_I64}
+
+
+def _plan_sizes(tokens, topk, num_experts):
+  """Refuses the sizes of a plan that are not served."""
+  if topk < 1 or topk > MOST_INT or not 1 <= num_experts <= MAX_EXPERTS:
+    raise invalid(f"an expert plan needs topk >= 1 and 1 to {MAX_EXPERTS} "
+                  "experts")
+  if tokens * topk > MOST_INT:
+    raise invalid("an expert plan holds less than 2^31 pairs")
 
 
 class ExpertPlan:
@@ -48,6 +57,7 @@ class ExpertPlan:
         offsets.numel() < 2:
       raise invalid("a plan has slots [tokens, topk], order [tokens * topk] "
                     "and offsets [num_experts + 1]")
+    _plan_sizes(*slots.shape, offsets.numel() - 1)
     if not offsets.device == order.device == slots.device:
       raise invalid("a plan's tensors lie on one device")
     self._offsets, self._order, self._slots = offsets, order, slots
@@ -96,9 +106,7 @@ class ExpertPlan:
   def empty(cls, tokens, topk, num_experts, device="cuda"):
     """A plan to be filled, on a device or that of a tensor; its arrays (slots,
     order, offsets, each on a 16-byte boundary) share one allocation."""
-    if topk < 1 or not 1 <= num_experts <= MAX_EXPERTS:
-      raise invalid(f"an expert plan needs topk >= 1 and 1 to {MAX_EXPERTS} "
-                    "experts")
+    _plan_sizes(tokens, topk, num_experts)
     part = _quads(tokens * topk)
     self = cls.__new__(cls)
     self._buffer = new_like(device, 2 * part + num_experts + 1, torch.int32)

@@ -43,6 +43,9 @@ def invalid(message):
   return C.XseError(C.INVALID_ARGUMENT, message)
 
 
+MOST_INT = 2 ** 31 - 1  # of the C ABI's 32-bit sizes; ctypes would cut larger ones
+
+
 def float_code(t, what):
   """XSE_DT_* of a float32 or bfloat16 CUDA tensor."""
   code = _FLOATS.get(t.dtype)
@@ -63,6 +66,8 @@ def matrix(t, what, rows=None):
   n, cols = shape
   if rows is not None and n != rows:
     raise invalid(f"{what} must have {rows} rows, got shape {tuple(shape)}")
+  if cols > MOST_INT:
+    raise invalid(f"{what} has {cols} columns: less than 2^31 are served")
   stride, step = t.stride()
   if cols > 1 and step != 1:
     raise invalid(f"{what} needs unit column stride")
@@ -104,6 +109,14 @@ def same_device(index, *tensors):
       raise invalid(f"tensors on {t.device} and device {index} in one call")
 
 
+def _matrix_sizes(rows, cols, groups):
+  """Refuses the sizes of a 4-bit matrix that are not served."""
+  if not 0 <= rows <= MOST_INT or not 1 <= cols <= 2 ** 30 or \
+      not 1 <= groups <= MOST_INT:
+    raise invalid("4-bit matrix needs 0 <= rows < 2^31, 1 <= cols <= 2^30 "
+                  "and 1 <= groups < 2^31.")
+
+
 class MxMatrix:
   """`groups` matrices of [rows, cols] in 4 bits (xse_mx_matrix): codes and
   scales are uint8 tensors of xse_mxfp4_codes_bytes and
@@ -113,6 +126,7 @@ class MxMatrix:
                "ref")
 
   def __init__(self, codes, scales, rows, cols, groups=1):
+    _matrix_sizes(rows, cols, groups)
     for name, t, need in (
         ("codes", codes, C.lib.xse_mxfp4_codes_bytes(rows, cols, groups)),
         ("scales", scales, C.lib.xse_mxfp4_scales_bytes(rows, cols, groups))):
@@ -156,9 +170,7 @@ class MxMatrix:
   def empty(cls, rows, cols, groups=1, device="cuda"):
     """A matrix to be filled, on a device or that of a tensor; codes and scales
     share one allocation."""
-    if rows < 0 or rows >= 2 ** 31 or not 1 <= cols <= 2 ** 30 or groups < 1:
-      raise invalid("4-bit matrix needs 0 <= rows < 2^31, 1 <= cols <= 2^30 "
-                    "and groups >= 1.")
+    _matrix_sizes(rows, cols, groups)
     at = groups * rows * ((cols + 31) // 32 * 16)  # a multiple of 16
     self = cls.__new__(cls)
     size = at + groups * ((rows + 127) // 128) * ((cols + 127) // 128) * 512
