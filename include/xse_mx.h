@@ -46,7 +46,8 @@ typedef struct xse_mx_matrix {
   int32_t groups;
 } xse_mx_matrix;
 
-/* Bytes of the two buffers (0 for sizes that are not served). */
+/* Bytes of the two buffers (0 for sizes that are not served: out of range, or of
+ * 2^63 bytes or more). */
 int64_t xse_mxfp4_codes_bytes(int64_t rows, int32_t cols, int32_t groups);
 int64_t xse_mxfp4_scales_bytes(int64_t rows, int32_t cols, int32_t groups);
 

@@ -2,9 +2,11 @@
 without a GPU: every refusal comes before the first CUDA call."""
 
 import ctypes
+import types
 
 import numpy as np
 import pytest
+import torch
 
 from tests import mx_reference as ref
 
@@ -106,6 +108,35 @@ def test_matrix_refusals(capi):
   refused(capi, d(matrix(capi), out=None), "null")
   assert q(matrix(capi, rows=0, codes=None, scales=None)) == capi.OK
   assert d(matrix(capi, rows=0, codes=None, scales=None)) == capi.OK
+
+
+@pytest.mark.parametrize("rows,cols,groups", [
+    (2 ** 30, 512, 2 ** 30),        # both sizes a multiple of 2^64
+    (2 ** 30, 2 ** 29, 1024),
+    (2 ** 30, 32, 2 ** 30), (2 ** 31 - 1, 2 ** 30, 2 ** 31 - 1),
+    (2 ** 31 - 1, 2 ** 30, 9)])
+def test_matrices_past_63_bits(capi, xse, rows, cols, groups):
+  """Their bytes have no number: nobody can have allocated them."""
+  lib = capi.lib
+  assert groups * rows * -(-cols // 32) * 16 >= 2 ** 63
+  assert lib.xse_mxfp4_codes_bytes(rows, cols, groups) == 0
+  assert lib.xse_mxfp4_scales_bytes(rows, cols, groups) == 0
+  q = matrix(capi, rows, cols, groups)
+  refused(capi, lib.xse_mxfp4_quantize(4096, 0, 0, 0, 0, q, None), "2^63")
+  refused(capi, lib.xse_mxfp4_dequantize(q, 4096, 0, 0, cols, None), "2^63")
+  buffer = types.SimpleNamespace(
+      dtype=torch.uint8, is_contiguous=lambda: True, is_cuda=True,
+      numel=lambda: 4096, device="cuda:0", data_ptr=lambda: 4096,
+      get_device=lambda: 0)
+  with pytest.raises(xse.XseError, match="2.63"):
+    xse.mx.MxMatrix(buffer, buffer, rows, cols, groups)
+
+
+def test_the_largest_sizes(capi):
+  rows, cols = 2 ** 31 - 1, 2 ** 30
+  assert capi.lib.xse_mxfp4_codes_bytes(rows, cols, 7) == 7 * rows * 2 ** 29
+  assert capi.lib.xse_mxfp4_scales_bytes(rows, cols, 7) == \
+      7 * 2 ** 24 * 2 ** 23 * 512
 
 
 def test_layer_refusals(capi):

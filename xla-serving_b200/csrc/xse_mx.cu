@@ -34,11 +34,12 @@ int LaunchStatus(const char* what) {
 }
 
 int CheckMxMatrix(const xse_mx_matrix* q, const char* what) {
-  if (q == nullptr || q->rows < 0 || q->cols < 1 || q->groups < 1 ||
-      q->rows > INT32_MAX || q->cols > kMostColumns) {
+  int64_t codes = 0, scales = 0;
+  if (q == nullptr ||
+      !MxMatrixBytes(q->rows, q->cols, q->groups, &codes, &scales)) {
     return FailWith(XSE_INVALID_ARGUMENT,
-                    "4-bit matrix %s needs 0 <= rows < 2^31, 1 <= cols <= 2^30 "
-                    "and groups >= 1.", what);
+                    "4-bit matrix %s needs 0 <= rows < 2^31, 1 <= cols <= "
+                    "2^30, groups >= 1 and less than 2^63 bytes.", what);
   }
   if (q->rows == 0) return XSE_OK;
   if (q->codes == nullptr || q->scales == nullptr) {
@@ -576,20 +577,15 @@ int QuantizeRows(const void* x, int32_t dtype, int64_t rows, int32_t cols,
 extern "C" {
 
 int64_t xse_mxfp4_codes_bytes(int64_t rows, int32_t cols, int32_t groups) {
-  if (rows < 0 || rows > INT32_MAX || cols < 1 || cols > xse::kMostColumns ||
-      groups < 1) {
-    return 0;
-  }
-  return groups * rows * xse::MxRowBytes(cols);
+  int64_t codes = 0, scales = 0;
+  xse::MxMatrixBytes(rows, cols, groups, &codes, &scales);
+  return codes;
 }
 
 int64_t xse_mxfp4_scales_bytes(int64_t rows, int32_t cols, int32_t groups) {
-  if (rows < 0 || rows > INT32_MAX || cols < 1 || cols > xse::kMostColumns ||
-      groups < 1) {
-    return 0;
-  }
-  return groups * xse::MxRowTiles(rows) * xse::MxKTiles(cols) *
-         xse::kMxTileBytes;
+  int64_t codes = 0, scales = 0;
+  xse::MxMatrixBytes(rows, cols, groups, &codes, &scales);
+  return scales;
 }
 
 int xse_mxfp4_quantize(const void* x, int32_t dtype, int64_t group_stride,

@@ -32,6 +32,26 @@ inline int64_t MxRowBytes(int64_t cols) { return (cols + 31) / 32 * 16; }
 inline int64_t MxKTiles(int64_t cols) { return (cols + 127) / 128; }
 inline int64_t MxRowTiles(int64_t rows) { return (rows + 127) / 128; }
 
+// Bytes of a matrix's codes and scales, false for sizes that are not served:
+// out of range, or with 2^63 bytes or more.
+inline bool MxMatrixBytes(int64_t rows, int64_t cols, int64_t groups,
+                          int64_t* codes, int64_t* scales) {
+  *codes = *scales = 0;
+  if (rows < 0 || rows > INT32_MAX || cols < 1 || cols > kMostColumns ||
+      groups < 1 || groups > INT32_MAX) {
+    return false;
+  }
+  // Of one group: below 2^60 and 2^56.
+  const int64_t group_codes = rows * MxRowBytes(cols);
+  const int64_t group_scales =
+      MxRowTiles(rows) * MxKTiles(cols) * kMxTileBytes;
+  const int64_t most = group_codes > group_scales ? group_codes : group_scales;
+  if (most > INT64_MAX / groups) return false;
+  *codes = groups * group_codes;
+  *scales = groups * group_scales;
+  return true;
+}
+
 inline bool Aligned16(const void* p) {
   return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 }

@@ -130,6 +130,8 @@ class MxMatrix:
     for name, t, need in (
         ("codes", codes, C.lib.xse_mxfp4_codes_bytes(rows, cols, groups)),
         ("scales", scales, C.lib.xse_mxfp4_scales_bytes(rows, cols, groups))):
+      if rows > 0 and need == 0:
+        raise invalid("4-bit matrix needs less than 2^63 bytes")
       if t.dtype != torch.uint8 or not t.is_contiguous() or \
           t.numel() < need or not t.is_cuda:
         raise invalid(f"4-bit matrix {name}: {need} contiguous uint8 bytes on "
