@@ -275,6 +275,44 @@ def test_linear_with_even_and_extreme_groups(mx, experts, cols):
     assert (np.abs(y.double().cpu().numpy() - want) <= bound).all()
 
 
+# tokens, topk, experts, in, out: three tiles or more for every block, in
+# uneven groups, for products in tiles of 16, 32, 64 and 128 rows and by pairs
+# of blocks.
+MANY_TILES = [
+    (200, 2, 40, 300, 2000), (500, 2, 40, 300, 2000), (1500, 1, 30, 700, 2000),
+    (6000, 2, 20, 300, 1000), (6000, 2, 20, 1600, 1000),
+    (6000, 2, 20, 1600, 900)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,topk,num_experts,cols,out", MANY_TILES)
+def test_linear_of_many_tiles(mx, experts, tokens, topk, num_experts, cols, out,
+                              dtype):
+  """Against 64 bits (summed on the device)."""
+  ids = choose(tokens, topk, num_experts, seed=10)
+  plan = experts.sort(torch.from_numpy(ids).cuda(), num_experts)
+  offsets, order, _ = ref.sort(ids, num_experts)
+  w, values = expert_weights(mx, num_experts, out, cols)
+  bias = make(num_experts, out, torch.float32, 2)
+  x = make(tokens, cols, dtype, 1)
+  q = torch.from_numpy(ref.quantized(x.double().numpy())).cuda()
+  rows = torch.from_numpy(np.maximum(order, 0) // topk).cuda()
+  outputs = [experts.linear(x.cuda(), plan, w, bias.cuda(), mx.ACT_RELU),
+             experts.linear(x.cuda()[rows], plan, w, bias.cuda(), mx.ACT_RELU,
+                            sorted_rows=True)]
+  assert torch.equal(*outputs)
+  for e in range(num_experts):
+    mine = slice(offsets[e], offsets[e + 1])
+    v, b = torch.from_numpy(values[e]).cuda(), bias[e].double().cuda()
+    want = torch.relu(q[rows[mine]] @ v.t() + b)
+    size = q[rows[mine]].abs() @ v.abs().t() + b.abs()
+    bound = (ref.linear_tolerance(0.0, size, cols, EPS[dtype]) +
+             EPS[dtype] / 2 * want)
+    assert bool(((outputs[0][mine].double() - want).abs() <= bound).all())
+  assert bool((outputs[0][offsets[-1]:] == 0).all())
+  mx.check()
+
+
 def mixture(mx, experts, ids, x, w1, b1, w2, b2, weights, num_experts):
   plan = experts.sort(ids, num_experts)
   h = experts.linear(x, plan, w1, b1, mx.ACT_RELU)
@@ -425,6 +463,30 @@ def test_offsets_past_32_bits(experts):
   assert torch.equal(gy[some], rows[some] * 2)
   want = (x[-5:].double() ** 2).sum(1, keepdim=True).expand(-1, topk)
   assert torch.equal(gw[-5:].double(), want)  # integers below 2^24
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_sort_of_millions(experts, dtype):
+  """More than 256 pairs a warp, some dropped: the stable order of torch's
+  sort, in which a dropped pair comes last."""
+  tokens, topk, num_experts = 300_000, 8, 130
+  gen = torch.Generator(device="cuda").manual_seed(1)
+  ids = torch.randint(-3, num_experts + 2, (tokens, topk), generator=gen,
+                      device="cuda").to(dtype)
+  plan = experts.sort(ids, num_experts)
+  flat = ids.view(-1).long()
+  key = torch.where((flat >= 0) & (flat < num_experts), flat, num_experts)
+  by = torch.sort(key, stable=True).indices
+  counts = torch.bincount(key, minlength=num_experts + 1)[:num_experts]
+  offsets = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+  kept = int(offsets[-1])
+  assert kept < flat.numel()
+  assert torch.equal(plan.offsets.long(), offsets)
+  assert torch.equal(plan.order[:kept].long(), by[:kept])
+  assert bool((plan.order[kept:] == -1).all())
+  slots = torch.full_like(flat, -1)
+  slots[by[:kept]] = torch.arange(kept, device="cuda")
+  assert torch.equal(plan.slots.view(-1).long(), slots)
 
 
 def out_weights(plan):

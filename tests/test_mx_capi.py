@@ -69,6 +69,25 @@ def test_expert_scale_tiles_never_overlap():
       assert last[-1] <= pairs // n + experts
 
 
+def test_expert_scale_tiles_of_pairs_never_overlap(capi):
+  """Tiles of 256 rows take two scale tiles of 128 rows each: an expert's rows
+  still have scale tiles of their own, and the workspace holds the last."""
+  rng = np.random.default_rng(2)
+  n, cols = 256, 1536
+  for _ in range(300):
+    experts = int(rng.integers(1, 40))
+    counts = rng.integers(0, 3 * n, experts) * (rng.random(experts) < 0.7)
+    offsets = np.concatenate([[0], np.cumsum(counts)])
+    pairs = int(offsets[-1] + rng.integers(0, 5))
+    first = (offsets[:-1] // n + np.arange(experts)) * 2
+    last = first + -(-counts // 128)
+    assert (last[:-1] <= first[1:]).all()
+    assert last[-1] <= (pairs // n + experts) * 2
+    if pairs > 128 * experts:  # the rule for such tiles
+      need = capi.lib.xse_expert_linear_workspace(pairs, experts, cols)
+      assert need >= pairs * cols // 2 + last[-1] * (cols // 128) * 512
+
+
 def test_reference_quantisation_by_search():
   """The reference's codes are a nearest grid value to the scaled element, the
   even one at a tie."""

@@ -226,6 +226,115 @@ def test_linear_repeats_bit_for_bit(mx):
       assert torch.equal(mx.linear(x, w), first)
 
 
+# rows, in, out: three tiles or more for every block, in each form of the
+# product (tiles of 16, 32, 64 and 128 rows, pairs of blocks with an even and an
+# odd number of feature tiles).
+MANY_TILES = [
+    (10, 500, 60_000), (30, 500, 60_001), (60, 700, 60_000), (2100, 300, 4000),
+    (2100, 1600, 6400), (2100, 1600, 6500)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,cols,out", MANY_TILES)
+def test_linear_of_many_tiles(mx, rows, cols, out, dtype):
+  """Against 64 bits (summed on the device: some 40 GFLOP)."""
+  x = make(rows, cols, dtype, seed=9)
+  w, w_values = weights(mx, out, cols)
+  gen = torch.Generator().manual_seed(out)
+  bias = torch.randn((out,), generator=gen)
+  y = mx.linear(x.cuda(), w, bias.cuda(), mx.ACT_RELU)
+  q = torch.from_numpy(ref.quantized(x.double().numpy())).cuda()
+  v, b = torch.from_numpy(w_values).cuda(), bias.double().cuda()
+  want = torch.relu(q @ v.t() + b)
+  size = q.abs() @ v.abs().t() + b.abs()
+  bound = (ref.linear_tolerance(0.0, size, cols, EPS[dtype]) +
+           EPS[dtype] / 2 * want)
+  assert bool(((y.double() - want).abs() <= bound).all())
+  again = mx.linear(x.cuda(), w, bias.cuda(), mx.ACT_RELU)
+  assert torch.equal(again, y)
+  mx.check()
+
+
+PAIRS = (300, 2048, 390)  # rows, in, out of a product by pairs of blocks
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pairs_strides_and_types(mx, dtype):
+  """Strided x and y (rows of y an even and an odd number of elements apart and
+  at odd offsets), the other output type, x quantised before: the numbers of
+  the plain call, and nothing outside y is written."""
+  rows, cols, out = PAIRS
+  x = make(rows, cols, dtype, seed=10)
+  w, _ = weights(mx, out, cols)
+  plain = mx.linear(x.cuda(), w)
+  exact = mx.linear(x.cuda(), w, out=torch.empty((rows, out), device="cuda"))
+  assert torch.equal(exact.to(dtype), plain)
+  buf = torch.zeros((rows, cols + 9), dtype=dtype, device="cuda")
+  buf[:, 5:5 + cols] = x.cuda()
+  for left, right in ((2, 4), (3, 3), (3, 4)):
+    y = torch.full((rows + 2, left + out + right), 7.0, dtype=dtype,
+                   device="cuda")
+    view = y[1:-1, left:left + out]
+    mx.linear(buf[:, 5:5 + cols], w, out=view)
+    assert torch.equal(view, plain)
+    view.fill_(7.0)
+    assert bool((y == 7.0).all())
+  q = mx.quantize(x.cuda())
+  assert torch.equal(mx.linear(q, w), exact)
+  half = torch.empty((rows, out), dtype=torch.bfloat16, device="cuda")
+  assert torch.equal(mx.linear(q, w, out=half), exact.bfloat16())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_pairs_keep_nan_in_its_row(mx, dtype):
+  rows, cols, out = PAIRS
+  x = make(rows, cols, dtype, seed=11)
+  w, w_values = weights(mx, out, cols)
+  bad = np.zeros(rows, bool)
+  for row, col, value in ((0, 0, "nan"), (127, 2047, "inf"), (128, 1024, "-inf"),
+                          (255, 31, "nan"), (256, 32, "inf"), (299, 5, "nan")):
+    x[row, col] = float(value)
+    bad[row] = True
+  y = mx.linear(x.cuda(), w, None, mx.ACT_RELU).double().cpu().numpy()
+  assert np.isnan(y[bad]).all()
+  want, size = ref.linear(x.double().numpy()[~bad], w_values, None, 1)
+  bound = ref.linear_tolerance(want, size, cols, EPS[dtype])
+  assert (np.abs(y[~bad] - want) <= bound).all()
+
+
+def test_pairs_on_other_streams_and_in_graphs(mx):
+  """Repeats, two streams at once, and two graphs replayed together."""
+  rows, cols, out = PAIRS
+  w, _ = weights(mx, out, cols)
+  xs = [make(n, cols, torch.bfloat16, seed=12 + n).cuda()
+        for n in (rows, 2000)]
+  want = [mx.linear(x, w) for x in xs]
+  torch.cuda.synchronize()
+  streams = [torch.cuda.Stream() for _ in xs]
+  for _ in range(20):
+    got = [mx.linear(x, w, stream=s) for x, s in zip(xs, streams)]
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+      assert torch.equal(a, b)
+  graphs, outs = [], []
+  for x in xs:
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+      outs.append(mx.linear(x, w))
+    graphs.append(g)
+  for _ in range(5):
+    for o in outs:
+      o.zero_()
+    torch.cuda.synchronize()
+    for g, s in zip(graphs, streams):
+      with torch.cuda.stream(s):
+        g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(outs, want):
+      assert torch.equal(a, b)
+  mx.check()
+
+
 def test_linear_empty(mx):
   w, _ = weights(mx, 64, 96)
   y = mx.linear(torch.zeros((0, 96), device="cuda"), w)
