@@ -111,8 +111,8 @@ def same_device(index, *tensors):
 
 def _matrix_sizes(rows, cols, groups):
   """Refuses the sizes of a 4-bit matrix that are not served."""
-  if not 0 <= rows <= MOST_INT or not 1 <= cols <= 2 ** 30 or \
-      not 1 <= groups <= MOST_INT:
+  if not (0 <= rows <= MOST_INT and 1 <= cols <= 2 ** 30 and
+          1 <= groups <= MOST_INT):
     raise invalid("4-bit matrix needs 0 <= rows < 2^31, 1 <= cols <= 2^30 "
                   "and 1 <= groups < 2^31.")
 
