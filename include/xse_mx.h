@@ -32,7 +32,8 @@ extern "C" {
 /* `groups` matrices of [rows, cols] in 4 bits (rows < 2^31, cols <= 2^30), as
  * one allocation each of codes and scales:
  *   codes: [groups][rows][16 * ceil(cols / 32)] bytes, element 2i in the low
- *          half of byte i; 16-byte aligned
+ *          half of byte i; 16-byte aligned. Codes past the last column are 0
+ *          (xse_mxfp4_quantize writes them).
  *   scales: [groups][ceil(rows / 128)][ceil(cols / 128)][512] bytes; block b
  *          of row r lies in tile (r / 128, b / 4) at byte
  *          (r % 32) * 16 + (r % 128) / 32 * 4 + b % 4; 16-byte aligned.
@@ -59,8 +60,10 @@ int xse_mxfp4_quantize(const void* x, int32_t dtype, int64_t group_stride,
                        int64_t row_stride, int64_t col_stride,
                        const xse_mx_matrix* q, void* stream);
 
-/* out = the values q stands for (exact in XSE_DT_F32 and XSE_DT_BF16), row r
- * of group g at out + g * group_stride + r * row_stride, row_stride >= cols. */
+/* out = the values q stands for (exact in XSE_DT_F32 and XSE_DT_BF16 for the
+ * scales that xse_mxfp4_quantize gives, up to 252; with 253 and 254 the largest
+ * codes pass the types' range and give infinities), row r of group g at
+ * out + g * group_stride + r * row_stride, row_stride >= cols. */
 int xse_mxfp4_dequantize(const xse_mx_matrix* q, void* out, int32_t dtype,
                          int64_t group_stride, int64_t row_stride,
                          void* stream);

@@ -400,8 +400,10 @@ __global__ void __launch_bounds__(kThreads)
 
 // Rings. A thread copies its 16 bytes of up to kC choices' rows into slots of
 // its own in shared memory with cp.async, several steps ahead of the step it
-// adds up: about 190 KB of rows are in flight per SM without holding a
-// register, and no thread waits for another.
+// adds up, without holding a register, and no thread waits for another. The ring
+// holds min(24 / kC, 8) steps of kC choices, kC the next of 1, 2, 4 and 8: 192 KB
+// of rows per SM for 4 choices and for 8, 144 KB for 3 (whose fourth slot stays
+// empty), 128 KB for 2, 64 KB for 1.
 constexpr int kRingThreads = 512;
 constexpr int kRingSlots = 24;  // 16-byte slots per thread
 constexpr int kRingBytes = kRingThreads * kRingSlots * 16;

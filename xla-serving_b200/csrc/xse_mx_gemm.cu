@@ -963,8 +963,9 @@ __launch_bounds__(std::is_void_v<X> ? kThreads : kThreadsWithRows, 1)
 // the pair's MMAs (issued by its first block) read both halves. An SM takes in
 // 64 bytes a cycle from L2 and moves 128 through its shared memory, and both
 // bound the products: the pair's 35 KB a stage need 560 cycles against its
-// MMAs' 512, a block by itself 51 KB for 128 x 256 (8192 x 4096 -> 8192: 114 us,
-// in pairs 104 us). Every block has its own accumulator, scales and epilogue.
+// MMAs' 512, a block by itself 51 KB for 128 x 256 (8192 x 4096 -> 8192 under the
+// power cap: 114 us, in pairs 104 us; off it, at 1.9 GHz, the pairs take 93 us).
+// Every block has its own accumulator, scales and epilogue.
 struct Pair {
   static constexpr int kN = 256;
   static constexpr int kBBytes = kN / 2 * kStageK / 2;

@@ -84,8 +84,11 @@ int CheckExpertPlan(const xse_expert_plan* plan);
 // many rows each, so that every tile's scales begin a column of tensor memory.
 // 256 rows (pairs of SMs) need a k that is long against the end of a tile,
 // which nothing overlaps there: 8192 rows to 8192 features in bf16, tiles of 128
-// and 256 rows, quantisation included: k 1024 60 and 68 us, k 2048 85 and 75 us,
-// k 4096 146 and 121 us; 64 experts' 512 rows each, k 2048: 111 and 106 us.
+// and 256 rows, quantisation included, both sides in turn with pauses (at 1.85 to
+// 1.97 GHz, off the power cap): k 1024 62 and 69 us, k 1536 72 and 75 us, k 2048
+// 87 and 78 us, k 4096 150 and 111 us; 64 experts of about 512 rows each, k 2048:
+// 111 and 102 us. The rule sees the average alone: where one group holds most of
+// the rows, its tiles are smaller than its own rows would ask for.
 inline int MxTileRowsFor(int64_t rows, int32_t groups, int32_t k) {
   const int64_t mean = (rows + groups - 1) / groups;
   if (mean <= 64) return mean <= 16 ? 16 : mean <= 32 ? 32 : 64;
